@@ -1147,6 +1147,256 @@ void sample_topp(torch::Tensor logits, torch::Tensor temperature, torch::Tensor 
                        out_tok.data_ptr<int64_t>(), stream()));
 }
 
+// ------------------------------------------- page-scaled 8-bit KV cache
+// kv_dtype number of a page-scaled cache; checks its tensors against each other.
+int page_cache(const char* op, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ks,
+               const torch::Tensor& vs, int64_t Hkv, int64_t Dh, int64_t page) {
+  const auto dt = k.scalar_type();
+  TORCH_CHECK(k.is_cuda() && (dt == torch::kFloat8_e4m3fn || dt == torch::kChar), op,
+              ": the cache must be a CUDA float8_e4m3fn or int8 tensor");
+  need_contig(v, "v_cache", dt);
+  need_contig(ks, "k_scale", torch::kFloat32);
+  need_contig(vs, "v_scale", torch::kFloat32);
+  TORCH_CHECK(k.is_contiguous(), op, ": k_cache must be contiguous");
+  TORCH_CHECK(Hkv > 0 && page > 0 && (Dh == 64 || Dh == 128), op, ": head_dim must be 64 or 128");
+  const int64_t slots = k.numel() / (Hkv * Dh);
+  TORCH_CHECK(k.numel() == v.numel() && slots * Hkv * Dh == k.numel() && slots % page == 0 && slots < (1ll << 31), op,
+              ": k_cache and v_cache are [pages * page, Hkv, Dh] of fewer than 2^31 slots");
+  TORCH_CHECK(ks.numel() == slots / page * Hkv && vs.numel() == ks.numel(), op, ": scales are [pages, Hkv]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
+              op, ": the cache must be 16-byte aligned");
+  return dt == torch::kFloat8_e4m3fn ? 1 : 2;
+}
+
+void same_device(const char* op, const torch::Tensor& a, std::initializer_list<const torch::Tensor*> others) {
+  for (const torch::Tensor* t : others)
+    TORCH_CHECK(t->device() == a.device(), op, ": tensors are on ", a.device().str(), " and ", t->device().str());
+}
+
+void page_append(torch::Tensor qkv, int64_t Hq, int64_t Hkv, int64_t Dh, torch::Tensor slots, torch::Tensor k_cache,
+                 torch::Tensor v_cache, torch::Tensor k_scale, torch::Tensor v_scale, int64_t page,
+                 torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(qkv.device());
+  need(qkv, "qkv", torch::kBFloat16);
+  TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && Hq >= 0 && qkv.size(1) == (Hq + 2 * Hkv) * Dh,
+              "page_append: qkv must be row-major [T, (Hq + 2 Hkv) * Dh]");
+  need_contig(slots, "slots", torch::kInt32);
+  TORCH_CHECK(slots.numel() == qkv.size(0), "page_append: one slot per row");
+  LkPageAppendDesc d{};
+  d.kv_dtype = page_cache("page_append", k_cache, v_cache, k_scale, v_scale, Hkv, Dh, page);
+  same_device("page_append", qkv, {&slots, &k_cache, &v_cache, &k_scale, &v_scale, &status});
+  d.qkv = qkv.data_ptr(); d.ld = qkv.stride(0); d.T = (int)qkv.size(0);
+  d.Hq = (int)Hq; d.Hkv = (int)Hkv; d.Dh = (int)Dh; d.page = (int)page;
+  d.slots = slots.data_ptr<int>();
+  d.k_cache = k_cache.data_ptr(); d.v_cache = v_cache.data_ptr();
+  d.k_scale = k_scale.data_ptr<float>(); d.v_scale = v_scale.data_ptr<float>();
+  d.num_slots = (int)(k_cache.numel() / (Hkv * Dh));
+  d.status = status.data_ptr<int>();
+  check(lk_page_append(&d, stream()));
+}
+
+void page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale, torch::Tensor v_scale,
+                 torch::Tensor slots, int64_t Hkv, int64_t Dh, int64_t page, torch::Tensor out, torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(out.device());
+  need_contig(slots, "slots", torch::kInt32);
+  need(out, "out", torch::kBFloat16);
+  TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == slots.numel() && out.size(1) == 2 * Hkv * Dh,
+              "page_gather: out must be row-major [n, 2 * Hkv * Dh]");
+  LkPageGatherDesc d{};
+  d.kv_dtype = page_cache("page_gather", k_cache, v_cache, k_scale, v_scale, Hkv, Dh, page);
+  same_device("page_gather", out, {&slots, &k_cache, &v_cache, &k_scale, &v_scale, &status});
+  d.k_cache = k_cache.data_ptr(); d.v_cache = v_cache.data_ptr();
+  d.k_scale = k_scale.data_ptr<float>(); d.v_scale = v_scale.data_ptr<float>();
+  d.slots = slots.data_ptr<int>();
+  d.n = (int)slots.numel(); d.Hkv = (int)Hkv; d.Dh = (int)Dh; d.page = (int)page;
+  d.num_slots = (int)(k_cache.numel() / (Hkv * Dh));
+  d.out = out.data_ptr(); d.ldo = out.stride(0);
+  d.status = status.data_ptr<int>();
+  check(lk_page_gather(&d, stream()));
+}
+
+torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,
+                             torch::Tensor v_scale, torch::Tensor tables, torch::Tensor ctx_lens, int64_t page,
+                             int64_t Hq, int64_t Hkv, int64_t Dh, int64_t q_len, int64_t max_ctx, double scale,
+                             c10::optional<torch::Tensor> out_opt, torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(q.device());
+  need(q, "q", torch::kBFloat16);
+  LkPageAttnDesc d{};
+  d.kv_dtype = page_cache("page_attention", k_cache, v_cache, k_scale, v_scale, Hkv, Dh, page);
+  TORCH_CHECK(Hq > 0 && Hq % Hkv == 0, "page_attention: Hq must be a multiple of Hkv");
+  TORCH_CHECK(q_len > 0 && q.dim() == 2 && q.stride(1) == 1 && q.size(1) == Hq * Dh && q.size(0) % q_len == 0,
+              "page_attention: q must be row-major [sequences * q_len, Hq * Dh]");
+  const int64_t n = q.size(0) / q_len;
+  need_contig(tables, "block_tables", torch::kInt32);
+  need_contig(ctx_lens, "ctx_lens", torch::kInt32);
+  TORCH_CHECK(tables.dim() == 2 && tables.size(0) == n && ctx_lens.numel() == n,
+              "page_attention: one table row and one length per sequence");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && (q.stride(0) % 8 == 0 || q.size(0) <= 1),
+              "page_attention: the rows of q must be 16-byte aligned");
+  torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({q.size(0), Hq * Dh}, q.options());
+  need(out, "out", torch::kBFloat16);
+  TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == q.size(0) && out.size(1) == Hq * Dh,
+              "page_attention: out must be row-major [sequences * q_len, Hq * Dh]");
+  same_device("page_attention", q, {&k_cache, &v_cache, &k_scale, &v_scale, &tables, &ctx_lens, &out, &status});
+  d.q = q.data_ptr(); d.ldq = q.stride(0);
+  d.k_cache = k_cache.data_ptr(); d.v_cache = v_cache.data_ptr();
+  d.k_scale = k_scale.data_ptr<float>(); d.v_scale = v_scale.data_ptr<float>();
+  d.tables = tables.data_ptr<int>(); d.ctx_lens = ctx_lens.data_ptr<int>();
+  d.max_pages = (int)tables.size(1); d.page = (int)page;
+  d.num_pages = (int)(k_cache.numel() / (Hkv * Dh) / page);
+  d.num_seqs = (int)n; d.q_len = (int)q_len;
+  d.Hq = (int)Hq; d.Hkv = (int)Hkv; d.Dh = (int)Dh;
+  d.scale = (float)scale;
+  d.out = out.data_ptr(); d.ldo = out.stride(0);
+  d.status = status.data_ptr<int>();
+  (void)max_ctx;
+  check(lk_page_attention(&d, stream()));
+  return out;
+}
+
+void copy_pages(std::vector<torch::Tensor> caches, torch::Tensor moves, int64_t num_pages, torch::Tensor status) {
+  TORCH_CHECK(!caches.empty() && caches.size() <= LK_COPY_TENSORS, "copy_pages: 1 to 8 tensors");
+  const c10::cuda::CUDAGuard g(caches[0].device());
+  need_contig(moves, "moves", torch::kInt32);
+  TORCH_CHECK(moves.dim() == 2 && moves.size(1) == 2, "copy_pages: moves must be [n, 2] (source, destination)");
+  TORCH_CHECK(num_pages > 0 && num_pages < (1ll << 31), "copy_pages: num_pages");
+  LkCopyPagesDesc d{};
+  d.layers = (int)caches[0].size(0);
+  for (size_t i = 0; i < caches.size(); ++i) {
+    const torch::Tensor& c = caches[i];
+    TORCH_CHECK(c.is_cuda() && c.is_contiguous() && c.dim() >= 2 && c.size(0) == d.layers && c.size(1) % num_pages == 0,
+                "copy_pages: caches must be contiguous CUDA tensors [layers, pages * rows, ...]");
+    same_device("copy_pages", caches[0], {&c, &moves, &status});
+    d.base[i] = c.data_ptr();
+    d.page_bytes[i] = d.layers ? c.numel() / d.layers / num_pages * c.element_size() : 0;
+  }
+  d.tensors = (int)caches.size();
+  d.num_pages = (int)num_pages;
+  d.num_moves = (int)moves.size(0);
+  d.moves = moves.data_ptr<int>();
+  d.status = status.data_ptr<int>();
+  check(lk_copy_pages(&d, stream()));
+}
+
+// ------------------------------------------- logits before sampling
+void row_table(const char* op, const torch::Tensor& counts) {
+  need(counts, "counts", torch::kInt16);
+  TORCH_CHECK(counts.dim() == 2 && counts.stride(1) == 1, op, ": counts must be row-major [rows, vocab]");
+}
+
+torch::Tensor adjust_logits(torch::Tensor logits, c10::optional<torch::Tensor> counts, c10::optional<torch::Tensor> rows,
+                            c10::optional<torch::Tensor> penalties, c10::optional<torch::Tensor> bias_offsets,
+                            c10::optional<torch::Tensor> bias_ids, c10::optional<torch::Tensor> bias_values,
+                            c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> mask_rows,
+                            c10::optional<torch::Tensor> out_opt, torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(logits.device());
+  const bool f32 = logits.scalar_type() == torch::kFloat32;
+  if (!f32) need(logits, "logits", torch::kBFloat16);
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
+              "adjust_logits: logits must be a row-major CUDA tensor [n, vocab]");
+  const int64_t n = logits.size(0), vocab = logits.size(1);
+  torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({n, vocab}, logits.options());
+  need(out, "out", logits.scalar_type());
+  TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == n && out.size(1) == vocab,
+              "adjust_logits: out must be row-major [n, vocab]");
+  same_device("adjust_logits", logits, {&out, &status});
+  LkAdjustLogitsDesc d{};
+  d.logits = logits.data_ptr(); d.ld = logits.stride(0);
+  d.out = out.data_ptr(); d.ldo = out.stride(0);
+  d.n = (int)n; d.vocab = (int)vocab; d.f32 = f32;
+  if (counts.has_value()) {
+    row_table("adjust_logits", *counts);
+    TORCH_CHECK(counts->size(1) == vocab, "adjust_logits: counts must have one column per token");
+    TORCH_CHECK(penalties.has_value(), "adjust_logits: counts need penalties");
+    need_contig(*penalties, "penalties", torch::kFloat32);
+    TORCH_CHECK(penalties->numel() == 3 * n, "adjust_logits: penalties must be [n, 3] (repetition, frequency, presence)");
+    same_device("adjust_logits", logits, {&*counts, &*penalties});
+    d.counts = counts->data_ptr<int16_t>(); d.ldc = counts->stride(0); d.count_rows = (int)counts->size(0);
+    d.penalties = penalties->data_ptr<float>();
+    if (rows.has_value()) {
+      need_contig(*rows, "rows", torch::kInt32);
+      TORCH_CHECK(rows->numel() == n, "adjust_logits: one counts row per logits row");
+      same_device("adjust_logits", logits, {&*rows});
+      d.rows = rows->data_ptr<int>();
+    } else {
+      TORCH_CHECK(counts->size(0) >= n, "adjust_logits: one counts row per logits row");
+    }
+  }
+  if (bias_offsets.has_value()) {
+    TORCH_CHECK(bias_ids.has_value() && bias_values.has_value(), "adjust_logits: bias is (offsets, ids, values)");
+    need_contig(*bias_offsets, "bias offsets", torch::kInt32);
+    need_contig(*bias_ids, "bias ids", torch::kInt32);
+    need_contig(*bias_values, "bias values", torch::kFloat32);
+    TORCH_CHECK(bias_offsets->numel() == n + 1 && bias_ids->numel() == bias_values->numel(),
+                "adjust_logits: bias offsets [n + 1], one value per id");
+    same_device("adjust_logits", logits, {&*bias_offsets, &*bias_ids, &*bias_values});
+    d.bias_offsets = bias_offsets->data_ptr<int>();
+    d.bias_ids = bias_ids->data_ptr<int>();
+    d.bias_values = bias_values->data_ptr<float>();
+    d.bias_count = (int)bias_ids->numel();
+  }
+  if (mask.has_value()) {
+    need(*mask, "mask", torch::kInt32);
+    TORCH_CHECK(mask->dim() == 2 && mask->stride(1) == 1 && mask->size(1) * 32 >= vocab,
+                "adjust_logits: mask must be row-major [rows, ceil(vocab / 32)]");
+    same_device("adjust_logits", logits, {&*mask});
+    d.mask = mask->data_ptr<int>(); d.ldm = mask->stride(0); d.mask_count = (int)mask->size(0);
+    if (mask_rows.has_value()) {
+      need_contig(*mask_rows, "mask_rows", torch::kInt32);
+      TORCH_CHECK(mask_rows->numel() == n, "adjust_logits: one mask row per logits row");
+      same_device("adjust_logits", logits, {&*mask_rows});
+      d.mask_rows = mask_rows->data_ptr<int>();
+    } else {
+      TORCH_CHECK(mask->size(0) >= n, "adjust_logits: one mask row per logits row");
+    }
+  }
+  d.status = status.data_ptr<int>();
+  check(lk_adjust_logits(&d, stream()));
+  return out;
+}
+
+void set_token_counts(torch::Tensor counts, c10::optional<torch::Tensor> rows, torch::Tensor tokens,
+                      torch::Tensor offsets, torch::Tensor prompt_lens, torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(counts.device());
+  row_table("set_token_counts", counts);
+  need_contig(tokens, "tokens", torch::kInt64);
+  need_contig(offsets, "offsets", torch::kInt32);
+  need_contig(prompt_lens, "prompt_lens", torch::kInt32);
+  const int64_t n = prompt_lens.numel();
+  TORCH_CHECK(offsets.numel() == n + 1, "set_token_counts: offsets [n + 1], prompt_lens [n]");
+  same_device("set_token_counts", counts, {&tokens, &offsets, &prompt_lens, &status});
+  LkTokenCountsDesc d{};
+  d.counts = counts.data_ptr<int16_t>(); d.ldc = counts.stride(0);
+  d.count_rows = (int)counts.size(0); d.vocab = (int)counts.size(1); d.n = (int)n;
+  if (rows.has_value()) {
+    need_contig(*rows, "rows", torch::kInt32);
+    TORCH_CHECK(rows->numel() == n, "set_token_counts: one row per history");
+    same_device("set_token_counts", counts, {&*rows});
+    d.rows = rows->data_ptr<int>();
+  }
+  d.tokens = tokens.data_ptr<int64_t>(); d.offsets = offsets.data_ptr<int>();
+  d.prompt_lens = prompt_lens.data_ptr<int>(); d.num_tokens = (int)tokens.numel();
+  d.status = status.data_ptr<int>();
+  check(lk_set_token_counts(&d, stream()));
+}
+
+void add_token_counts(torch::Tensor counts, c10::optional<torch::Tensor> rows, torch::Tensor tokens,
+                      torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(counts.device());
+  row_table("add_token_counts", counts);
+  need_contig(tokens, "tokens", torch::kInt64);
+  same_device("add_token_counts", counts, {&tokens, &status});
+  const int* r = nullptr;
+  if (rows.has_value()) {
+    need_contig(*rows, "rows", torch::kInt32);
+    TORCH_CHECK(rows->numel() == tokens.numel(), "add_token_counts: one row per token");
+    same_device("add_token_counts", counts, {&*rows});
+    r = rows->data_ptr<int>();
+  }
+  check(lk_add_token_counts(counts.data_ptr<int16_t>(), counts.stride(0), (int)counts.size(0), (int)counts.size(1), r,
+                            tokens.data_ptr<int64_t>(), (int)tokens.numel(), status.data_ptr<int>(), stream()));
+}
+
 void quantize(int64_t fmt, torch::Tensor w, int64_t group, torch::Tensor q, torch::Tensor scale,
               c10::optional<torch::Tensor> zero) {
   const c10::cuda::CUDAGuard g(w.device());
@@ -1224,6 +1474,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample", &sample);
   m.def("sample_topp", &sample_topp);
   m.def("kv_gather", &kv_gather);
+  m.def("page_append", &page_append);
+  m.def("page_gather", &page_gather);
+  m.def("page_attention", &page_attention);
+  m.def("copy_pages", &copy_pages);
+  m.def("adjust_logits", &adjust_logits);
+  m.def("set_token_counts", &set_token_counts);
+  m.def("add_token_counts", &add_token_counts);
   m.def("quantize", &quantize);
   m.def("dequant_gemv", &dequant_gemv);
   m.def("dequantize", &dequantize);

@@ -446,6 +446,107 @@ int lk_sample_topp(const void* logits, int64_t ld, int rows, int V, const float*
                    const float* top_p, uint64_t seed, const uint64_t* row_seeds, int64_t* out_tok,
                    cudaStream_t s);
 
+// ------------------------------------- page-scaled 8-bit KV cache (kv_page.cu)
+// Codes [num_slots, Hkv, Dh] (kv_dtype 1 = fp8 e4m3, 2 = int8), one power-of-two
+// fp32 scale per (page, KV head) [num_slots / page, Hkv]; slot = page id * page + offset.
+typedef struct LkPageAppendDesc {
+  const void* qkv;  // [T, (Hq+2Hkv)*Dh] bf16 (post-RoPE), row pitch ld
+  int64_t ld;
+  int T, Hq, Hkv, Dh, page;
+  const int* slots;  // [T], < 0 = skip; the new rows of one page are consecutive and ascending
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  int num_slots;
+  int kv_dtype;
+  int* status;
+} LkPageAppendDesc;
+int lk_page_append(const LkPageAppendDesc* d, cudaStream_t s);
+
+typedef struct LkPageGatherDesc {
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int* slots;  // [n]
+  int n, Hkv, Dh, page, num_slots;
+  void* out;         // [n, 2*Hkv*Dh] bf16: keys, then values; row pitch ldo
+  int64_t ldo;
+  int kv_dtype;
+  int* status;
+} LkPageGatherDesc;
+int lk_page_gather(const LkPageGatherDesc* d, cudaStream_t s);
+
+// Attention of the newest q_len tokens of each sequence (kv_page_attn.cu).
+typedef struct LkPageAttnDesc {
+  const void* q;  // [num_seqs * q_len, Hq*Dh] bf16, row pitch ldq
+  int64_t ldq;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int* tables;    // [num_seqs, max_pages] page ids
+  const int* ctx_lens;  // [num_seqs], the q_len newest tokens included
+  int max_pages, page, num_pages, num_seqs, q_len, Hq, Hkv, Dh;
+  float scale;
+  void* out;  // [num_seqs * q_len, Hq*Dh] bf16
+  int64_t ldo;
+  int kv_dtype;
+  int* status;
+} LkPageAttnDesc;
+int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s);
+
+// Copies page moves[2i] over page moves[2i+1] in every layer of every tensor
+// [layers, num_pages, page_bytes] (no destination is another move's source).
+#define LK_COPY_TENSORS 8
+typedef struct LkCopyPagesDesc {
+  void* base[LK_COPY_TENSORS];
+  int64_t page_bytes[LK_COPY_TENSORS];
+  int tensors, layers, num_pages, num_moves;
+  const int* moves;  // [num_moves, 2]
+  int* status;
+} LkCopyPagesDesc;
+int lk_copy_pages(const LkCopyPagesDesc* d, cudaStream_t s);
+
+// ----------------------------------------- logits before sampling (logits.cu)
+typedef struct LkAdjustLogitsDesc {
+  const void* logits;  // [n, vocab] bf16 or fp32, row pitch ld
+  void* out;           // same type, row pitch ldo (may be logits)
+  int64_t ld, ldo;
+  int n, vocab, f32;
+  const int16_t* counts;   // [count_rows, vocab], row pitch ldc; null = no penalties
+  int64_t ldc;
+  int count_rows;
+  const int* rows;         // [n] row of counts, < 0 = no penalties; null = i
+  const float* penalties;  // [n, 3] repetition, frequency, presence
+  const int* bias_offsets;  // [n + 1] or null
+  const int* bias_ids;
+  const float* bias_values;
+  int bias_count;
+  const int* mask;       // [mask_count, >= ceil(vocab / 32)] bit set = allowed, row pitch ldm; null = none
+  int64_t ldm;
+  int mask_count;
+  const int* mask_rows;  // [n] row of mask, < 0 = unrestricted; null = i
+  int* status;
+} LkAdjustLogitsDesc;
+int lk_adjust_logits(const LkAdjustLogitsDesc* d, cudaStream_t s);
+
+typedef struct LkTokenCountsDesc {
+  int16_t* counts;  // [count_rows, vocab], row pitch ldc
+  int64_t ldc;
+  int count_rows, vocab, n;
+  const int* rows;          // [n] row of counts, < 0 = skip; null = i
+  const int64_t* tokens;    // histories, concatenated
+  const int* offsets;       // [n + 1]
+  const int* prompt_lens;   // [n] leading tokens of each history that are its prompt
+  int num_tokens;
+  int* status;
+} LkTokenCountsDesc;
+int lk_set_token_counts(const LkTokenCountsDesc* d, cudaStream_t s);
+int lk_add_token_counts(int16_t* counts, int64_t ldc, int count_rows, int vocab, const int* rows,
+                        const int64_t* tokens, int n, int* status, cudaStream_t s);
+
 // ------------------------------------------------------ K14 quantised weights
 enum LkQuantFmt { LK_Q_INT8 = 0, LK_Q_FP8 = 1, LK_Q_INT4 = 2 };
 int lk_quantize(int fmt, const void* w, int N, int K, int group, void* q, float* scale, float* zero,
