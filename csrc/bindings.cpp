@@ -1249,7 +1249,16 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
   d.scale = (float)scale;
   d.out = out.data_ptr(); d.ldo = out.stride(0);
   d.status = status.data_ptr<int>();
-  (void)max_ctx;
+  if (max_ctx <= 0 || max_ctx > tables.size(1) * page) max_ctx = tables.size(1) * page;
+  TORCH_CHECK(max_ctx < (1ll << 31) - 64, "page_attention: contexts of fewer than 2^31 tokens");
+  d.nsplit = lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)max_ctx);
+  torch::Tensor part;  // allocated per call: the allocator knows the stream
+  if (d.nsplit > 1) {
+    const int64_t parts = q.size(0) * Hq * d.nsplit;
+    part = torch::empty({parts * (Dh + 4)}, q.options().dtype(torch::kFloat32));
+    d.part_ml = part.data_ptr<float>();
+    d.part_o = d.part_ml + parts * 4;
+  }
   check(lk_page_attention(&d, stream()));
   return out;
 }

@@ -6,6 +6,32 @@
 //
 // Query j of a sequence of ctx tokens sits at position ctx - q_len + j.  A query
 // without a token before it (an unused batch row of ctx 0) gives zeros.
+//
+// The cache is read once: 2 * Hkv * Dh bytes a token, against 4 * Hq * Dh flops
+// per query token, so HBM bounds it as long as the work per byte stays small.
+// On CUDA cores it does not (conversions, products and the reductions of the
+// scores cost more issue slots than the bytes bring), hence tensor cores, with
+// the tokens as the M dimension of both products so that the few query rows
+// (GQA group * q_len, columns of 8) waste nothing:
+//
+//   S^T [tokens x queries] = K Q^T      O^T [dims x queries] += V^T P^T
+//
+// mma.sync m16n8k16 in f16 with fp32 sums: a code is exact in f16 (e4m3 by one
+// conversion per two codes), and the fragments of K and of V^T are exactly what
+// 16-byte loads of the cached rows bring to each lane, the order of the
+// summed index being free (dims for K; a lane's dims are 16 neighbours of one
+// row).  tcgen05 would want both operands in 8 bits (the query rounded to them)
+// or the codes converted into shared memory first.  Each lane fills its own
+// slots of a ring with cp.async and reads them back itself: the asynchronous
+// copies need no barrier, and addresses are free, so any page size works and a
+// page may end inside a tile.
+//
+// Softmax per warp, one pass.  Weights are f16, so they are taken relative to
+// a running reference m with 2^7 at the largest one so far and moved only when
+// a score passes 2^14 (f16 ends at 2^16): weights down to 2^-31 of the largest
+// count.  A page's value scale 2^e enters as e added to the score, with a
+// reference of its own: a page of small values is then as exact as one of large
+// ones whichever the query looks at.  The softmax sum is kept in fp32 apart.
 #include "common.cuh"
 #include "host_util.h"
 #include "kv_page.cuh"
@@ -13,77 +39,467 @@
 
 namespace lk {
 
-// One block per (query row, query head); each warp takes every fourth token
-// with its lanes over the head dimension, and the four running softmaxes are
-// merged at the end.
-template <int KV, int DH>
-__global__ void __launch_bounds__(128) page_attn_kernel(LkPageAttnDesc d) {
-  constexpr int PER = DH / 32;
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][DH];
-  const int row = blockIdx.x, head = blockIdx.y;
-  const int seq = row / d.q_len, h = head / (d.Hq / d.Hkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int ctx = d.ctx_lens[seq];
-  if (ctx > (int64_t)d.max_pages * d.page) {
-    if (threadIdx.x == 0 && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-    ctx = d.max_pages * d.page;
+constexpr int PA_WARPS = 4;
+constexpr int PA_UNIT = 32;        // tokens a warp takes at a time (two M = 16 tiles)
+constexpr float PA_LOW = -3.0e38f;  // reference before the first token
+constexpr float PA_TOP = 14.f, PA_AIM = 7.f;
+
+template <int DH>
+struct PaRing {
+  static constexpr int KV_BYTES = PA_UNIT * DH;           // keys (or values) of a unit
+  static constexpr int SCALES = 2 * KV_BYTES;             // float2 (key, value scale) per token
+  static constexpr int MASK = SCALES + PA_UNIT * 8;       // bit per token: its page id is valid
+  static constexpr int STAGE = MASK + 16;
+  static constexpr int STAGES = 3;
+  static constexpr int WARP = STAGE * STAGES;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(on ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Codes of the low (HI = 0) or high two bytes of w as f16x2.  int8: byte ^ 0x80
+// under the exponent of 1024 is 1152 + code.
+template <int KV, int HI>
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
+  if constexpr (KV == 1) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? w >> 16 : w & 0xFFFFu), __NV_E4M3);
+    return (uint32_t)h.x | (uint32_t)h.y << 16;
+  } else {
+    const uint32_t u = __byte_perm(w ^ 0x80808080u, 0x64646464u, HI ? 0x4342 : 0x4140);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
-  const int upto = ctx - d.q_len + row % d.q_len + 1;
+}
+
+// What the blocks of a sequence's row tile share: the tokens [0, end) that any of
+// its queries sees, cut into nsplit parts of `per` units.
+struct PaSpan {
+  int ctx, end, units, per;
+};
+
+__device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int seq, int last_row, int group, int nsplit) {
+  PaSpan s;
+  s.ctx = (int)min((int64_t)max(d.ctx_lens[seq], 0), (int64_t)d.max_pages * d.page);
+  s.end = max(0, s.ctx - d.q_len + last_row / group + 1);
+  s.units = (s.end + PA_UNIT - 1) / PA_UNIT;
+  s.per = max((s.units + nsplit - 1) / nsplit, PA_WARPS);
+  return s;
+}
+
+// Grid: split fastest, then KV head, row tile (8 * NT query rows), sequence.
+template <int KV, int DH, int NT>
+__global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnDesc d, int tiles, int nsplit) {
+  using R = PaRing<DH>;
+  constexpr int ROWS = 8 * NT, CH = DH / 64, MT = DH / 16;
+  extern __shared__ __align__(16) uint8_t sm[];
+  const int split = blockIdx.x % nsplit;
+  int b = blockIdx.x / nsplit;
+  const int h = b % d.Hkv;
+  b /= d.Hkv;
+  const int tile = b % tiles, seq = b / tiles;
+  const int group = d.Hq / d.Hkv, rows = group * d.q_len;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const PaSpan sp = page_attn_span(d, seq, min(rows, (tile + 1) * ROWS) - 1, group, nsplit);
+  if (threadIdx.x == 0 && d.ctx_lens[seq] > (int64_t)d.max_pages * d.page && d.status)
+    atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
+  const int u_end = min(sp.units, (split + 1) * sp.per);
+  if (split > 0 && split * sp.per >= sp.units) return;
+
+  // this lane's tokens' addresses and this warp's ring
+  const int64_t tok_stride = (int64_t)d.Hkv * DH;
+  const uint8_t* kbase = (const uint8_t*)d.k_cache + h * DH;
+  const uint8_t* vbase = (const uint8_t*)d.v_cache + h * DH;
   const int* table = d.tables + (int64_t)seq * d.max_pages;
-  const __nv_bfloat16* q = (const __nv_bfloat16*)d.q + (int64_t)row * d.ldq + head * DH;
-  float qf[PER], o[PER], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < PER; ++i) {
-    qf[i] = __bfloat162float(q[i * 32 + lane]);
-    o[i] = 0.f;
-  }
-  const float sl2 = d.scale * 1.4426950408889634f;
-  for (int t = warp; t < upto; t += 4) {
-    const int pg = table[t / d.page];
-    if (pg < 0 || pg >= d.num_pages) {
-      if (lane == 0 && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-      continue;
+  uint8_t* ring = sm + warp * R::WARP;
+  const uint32_t ring_u = smem_u32(ring);
+
+  auto page_of = [&](int u) {
+    const int t = u * PA_UNIT + lane;
+    return u < u_end && t < sp.end ? table[t / d.page] : 0;
+  };
+  auto issue = [&](int u, int stage, int pg) {
+    if (u < u_end) {
+      const int t = u * PA_UNIT + lane;
+      bool ok = t < sp.end;
+      if (ok && (pg < 0 || pg >= d.num_pages)) {
+        if (d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
+        ok = false;
+      }
+      const int slot = ok ? pg * d.page + t % d.page : -1;
+      const uint32_t st = ring_u + stage * R::STAGE;
+      const unsigned valid = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) *reinterpret_cast<unsigned*>(ring + stage * R::STAGE + R::MASK) = valid;
+      const int64_t sc = ok ? (int64_t)pg * d.Hkv + h : 0;
+      cp_async4(st + R::SCALES + lane * 8, d.k_scale + sc, ok);
+      cp_async4(st + R::SCALES + lane * 8 + 4, d.v_scale + sc, ok);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // keys of tokens r, r + 8, r + 16, r + 24
+        const int s = __shfl_sync(0xffffffffu, slot, r + 8 * i);
+        const uint8_t* p = kbase + (s < 0 ? 0 : s) * tok_stride + c * 16;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) cp_async16(st + ((i * CH + k) * 32 + lane) * 16, p + 64 * k, s >= 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // values of tokens 2c, 2c + 1, 2c + 8, 2c + 9, then 16 on
+        const int s = __shfl_sync(0xffffffffu, slot, 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * c + (i & 1));
+        const uint8_t* p = vbase + (s < 0 ? 0 : s) * tok_stride + r * (DH / 8);
+        if constexpr (DH == 128) cp_async16(st + R::KV_BYTES + (i * 32 + lane) * 16, p, s >= 0);
+        else cp_async8(st + R::KV_BYTES + (i * 32 + lane) * 8, p, s >= 0);
+      }
     }
-    const int64_t at = (((int64_t)pg * d.page + t % d.page) * d.Hkv + h) * DH + lane;
-    float s = 0.f;
-    for (int i = 0; i < PER; ++i) s += qf[i] * page_decode<KV>(((const uint8_t*)d.k_cache)[at + i * 32]);
-    s = warp_sum(s) * sl2 * d.k_scale[(int64_t)pg * d.Hkv + h];
-    const float mn = fmaxf(m, s);
-    const float a = m == -INFINITY ? 0.f : exp2f(m - mn), p = exp2f(s - mn);
-    m = mn;
-    l = l * a + p;
-    const float pv = p * d.v_scale[(int64_t)pg * d.Hkv + h];
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * a + pv * page_decode<KV>(((const uint8_t*)d.v_cache)[at + i * 32]);
+    cp_commit();
+  };
+
+  // query fragments: column r of each tile, the dims of this lane's key bytes, times
+  // a power of two that brings the row's largest value to [2^7, 2^8) (f16 is then
+  // exact down to 2^-22 of it)
+  uint32_t qf[NT][4 * CH][2];
+  float qfac[NT][2];
+  int lim[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = tile * ROWS + n * 8 + r;
+    uint32_t w[8 * CH];
+#pragma unroll
+    for (int i = 0; i < 8 * CH; ++i) w[i] = 0;
+    if (row < rows) {
+      const uint4* p = reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.q +
+                                                      ((int64_t)seq * d.q_len + row / group) * d.ldq +
+                                                      (h * group + row % group) * DH);
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = p[k * 8 + c * 2 + i];
+          w[k * 8 + i * 4] = v.x, w[k * 8 + i * 4 + 1] = v.y, w[k * 8 + i * 4 + 2] = v.z, w[k * 8 + i * 4 + 3] = v.w;
+        }
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8 * CH; ++i) {
+      const float2 f = unpack_bf16x2(w[i]);
+      if (fabsf(f.x) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.x));
+      if (fabsf(f.y) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.y));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -119);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int k = 0; k < 4 * CH; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 f = unpack_bf16x2(w[2 * k + i]);
+        const __half2 hv = __floats2half2_rn(f.x * down, f.y * down);
+        qf[n][k][i] = *reinterpret_cast<const uint32_t*>(&hv);
+      }
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23) * (d.scale * 1.4426950408889634f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      qfac[n][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
+      const int col = tile * ROWS + n * 8 + 2 * c + i;
+      lim[n][i] = col < rows ? sp.ctx - d.q_len + col / group + 1 : sp.end;
+    }
   }
-  if (lane == 0) {
-    sm_m[warp] = m;
-    sm_l[warp] = l;
+  const int open = sp.ctx - d.q_len + tile * ROWS / group + 1;  // tokens that every query of the tile sees
+
+  float acc[NT][MT][4], ms[NT][2], mw[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][j][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ms[n][i] = mw[n][i] = PA_LOW, l[n][i] = 0.f;
   }
-  for (int i = 0; i < PER; ++i) sm_o[warp][i * 32 + lane] = o[i];
+
+  int u = split * sp.per + warp;
+#pragma unroll
+  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, page_of(u + s * PA_WARPS));
+  int pg = page_of(u + R::STAGES * PA_WARPS);
+  int stage = 0;
+  for (; u < u_end; u += PA_WARPS) {
+    cp_wait<R::STAGES - 1>();
+    __syncwarp();
+    const uint8_t* st = ring + stage * R::STAGE;
+    // scores of both 16-token tiles
+    float s[2][NT][4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[g][n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const uint4 x = *reinterpret_cast<const uint4*>(st + ((2 * g * CH + k) * 32 + lane) * 16);
+        const uint4 y = *reinterpret_cast<const uint4*>(st + (((2 * g + 1) * CH + k) * 32 + lane) * 16);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a0 = codes_f16x2<KV, 0>(xs[i]), a1 = codes_f16x2<KV, 0>(ys[i]);
+          const uint32_t a2 = codes_f16x2<KV, 1>(xs[i]), a3 = codes_f16x2<KV, 1>(ys[i]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(s[g][n], a0, a1, a2, a3, qf[n][4 * k + i][0], qf[n][4 * k + i][1]);
+        }
+      }
+    }
+    // scale, mask; the score plus the value scale's exponent is the weight's exponent
+    const unsigned valid = *reinterpret_cast<const unsigned*>(st + R::MASK);
+    const bool all = valid == 0xffffffffu && (u + 1) * PA_UNIT <= open;
+    float lv[2][2];
+    bool move = false;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int tl = 16 * g + 8 * i + r;
+        const float2 sc = *reinterpret_cast<const float2*>(st + R::SCALES + tl * 8);
+        lv[g][i] = __log2f(sc.y);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float x = s[g][n][2 * i + q] * sc.x * qfac[n][q];
+            if (!all && (u * PA_UNIT + tl >= lim[n][q] || !((valid >> tl) & 1))) x = -INFINITY;
+            s[g][n][2 * i + q] = x;
+            move |= x > ms[n][q] + PA_TOP || x + lv[g][i] > mw[n][q] + PA_TOP;
+          }
+      }
+    if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float a = -INFINITY, w = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              a = fmaxf(a, s[g][n][2 * i + q]);
+              w = fmaxf(w, s[g][n][2 * i + q] + lv[g][i]);
+            }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+          }
+          // a column moves by its own scores alone: its bits do not depend on its neighbours
+          if (a > ms[n][q] + PA_TOP) {
+            l[n][q] *= fast_exp2(ms[n][q] - (a - PA_AIM));
+            ms[n][q] = a - PA_AIM;
+          }
+          if (w > mw[n][q] + PA_TOP) {
+            const float f = fast_exp2(mw[n][q] - (w - PA_AIM));
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[n][j][q] *= f, acc[n][j][2 + q] *= f;
+            mw[n][q] = w - PA_AIM;
+          }
+        }
+    }
+    // weights, transposed from [tokens x queries] to the B operand
+    uint32_t p[2][NT][2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float w[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float x = s[g][n][2 * i + q];
+            l[n][q] += fast_exp2(x - ms[n][q]);
+            w[q] = fast_exp2(x + lv[g][i] - mw[n][q]);
+          }
+          const __half2 hv = __floats2half2_rn(w[0], w[1]);
+          p[g][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
+        }
+    // O^T += V^T P^T: tile j takes this lane's dims 2j and 2j + 1
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t v[4][DH / 32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DH == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(st + R::KV_BYTES + ((4 * g + i) * 32 + lane) * 16);
+          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(st + R::KV_BYTES + ((4 * g + i) * 32 + lane) * 8);
+          v[i][0] = x.x, v[i][1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < DH / 32; ++m)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const uint32_t ab = __byte_perm(v[0][m], v[1][m], o ? 0x7362 : 0x5140);
+          const uint32_t cd = __byte_perm(v[2][m], v[3][m], o ? 0x7362 : 0x5140);
+          const uint32_t a0 = codes_f16x2<KV, 0>(ab), a1 = codes_f16x2<KV, 1>(ab);
+          const uint32_t a2 = codes_f16x2<KV, 0>(cd), a3 = codes_f16x2<KV, 1>(cd);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * m + o], a0, a1, a2, a3, p[g][n][0], p[g][n][1]);
+        }
+    }
+    __syncwarp();  // every lane is done with the stage's scales and mask
+    issue(u + R::STAGES * PA_WARPS, stage, pg);
+    pg = page_of(u + (R::STAGES + 1) * PA_WARPS);
+    stage = stage + 1 == R::STAGES ? 0 : stage + 1;
+  }
+  cp_wait<0>();
   __syncthreads();
-  for (int c = threadIdx.x; c < DH; c += 128) {
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
-    for (int w = 0; w < 4; ++w) {
-      const float f = sm_m[w] == -INFINITY ? 0.f : exp2f(sm_m[w] - M);
-      L += sm_l[w] * f;
-      O += sm_o[w][c] * f;
+
+  // merge the warps: [warp][row][DH + 3] floats over the ring
+  float* part = reinterpret_cast<float*>(sm);
+  constexpr int PITCH = DH + 4;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      float x = l[n][q];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      float* row = part + (warp * ROWS + n * 8 + 2 * c + q) * PITCH;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        row[r * (DH / 8) + 2 * j] = acc[n][j][q];
+        row[r * (DH / 8) + 2 * j + 1] = acc[n][j][2 + q];
+      }
+      if (r == 0) row[DH] = ms[n][q], row[DH + 1] = mw[n][q], row[DH + 2] = x;
     }
-    ((__nv_bfloat16*)d.out)[(int64_t)row * d.ldo + head * DH + c] = __float2bfloat16(L == 0.f ? 0.f : O / L);
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * DH; i += 32 * PA_WARPS) {
+    const int rl = i / DH, dim = i % DH, row = tile * ROWS + rl;
+    if (row >= rows) break;
+    const float* x = part + rl * PITCH;
+    float MS = PA_LOW, MW = PA_LOW, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) {
+      MS = fmaxf(MS, x[w * ROWS * PITCH + DH]);
+      MW = fmaxf(MW, x[w * ROWS * PITCH + DH + 1]);
+    }
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) {
+      const float* y = x + w * ROWS * PITCH;
+      L += y[DH + 2] * fast_exp2(y[DH] - MS);
+      O += y[dim] * fast_exp2(y[DH + 1] - MW);
+    }
+    const int64_t grow = (int64_t)seq * d.q_len + row / group;
+    const int head = h * group + row % group;
+    if (nsplit == 1) {
+      O *= fast_exp2(MW - MS);
+      ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + dim] = __float2bfloat16(L == 0.f ? 0.f : O / L);
+    } else {
+      const int64_t at = (grow * d.Hq + head) * nsplit + split;
+      d.part_o[at * DH + dim] = O;
+      if (dim == 0) *reinterpret_cast<float4*>(d.part_ml + at * 4) = make_float4(MS, MW, L, 0.f);
+    }
   }
+}
+
+// Joins the parts of a (row, head): one warp each, in the order of the parts.
+template <int DH>
+__global__ void page_attn_join_kernel(LkPageAttnDesc d, int tile_rows, int nsplit) {
+  const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (w >= (int64_t)d.num_seqs * d.q_len * d.Hq) return;
+  const int64_t grow = w / d.Hq;
+  const int head = (int)(w % d.Hq), group = d.Hq / d.Hkv;
+  const int row = (int)(grow % d.q_len) * group + head % group;
+  const int last = min(group * d.q_len, (row / tile_rows + 1) * tile_rows) - 1;
+  const PaSpan sp = page_attn_span(d, (int)(grow / d.q_len), last, group, nsplit);
+  const int used = max(1, (sp.units + sp.per - 1) / sp.per);
+  const float4* ml = reinterpret_cast<const float4*>(d.part_ml) + w * nsplit;
+  float MS = PA_LOW, MW = PA_LOW, L = 0.f, o[DH / 32];
+  for (int s = 0; s < used; ++s) {
+    MS = fmaxf(MS, ml[s].x);
+    MW = fmaxf(MW, ml[s].y);
+  }
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i) o[i] = 0.f;
+  for (int s = 0; s < used; ++s) {
+    const float4 x = ml[s];
+    L += x.z * fast_exp2(x.x - MS);
+    const float f = fast_exp2(x.y - MW);
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) o[i] += d.part_o[(w * nsplit + s) * DH + i * 32 + lane] * f;
+  }
+  const float f = fast_exp2(MW - MS);
+#pragma unroll
+  for (int i = 0; i < DH / 32; ++i)
+    ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + i * 32 + lane] = __float2bfloat16(L == 0.f ? 0.f : o[i] * f / L);
+}
+
+template <int KV, int DH, int NT>
+static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
+  const int rows = d.Hq / d.Hkv * d.q_len, tiles = cdiv(rows, 8 * NT);
+  const int64_t blocks = (int64_t)d.num_seqs * d.Hkv * tiles * d.nsplit;
+  LK_REQUIRE(blocks < (1ll << 31), "page_attention: too many rows in one call");
+  constexpr int merge = PA_WARPS * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
+  constexpr int smem = ring > merge ? ring : merge;
+  auto k = page_attn_kernel<KV, DH, NT>;
+  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, tiles, d.nsplit);
+  if (check_launch("page_attention")) return -1;
+  if (d.nsplit == 1) return 0;
+  const int64_t warps = (int64_t)d.num_seqs * d.q_len * d.Hq;
+  page_attn_join_kernel<DH><<<cdiv(warps * 32, 128), 128, 0, s>>>(d, 8 * NT, d.nsplit);
+  return check_launch("page_attention_join");
 }
 
 }  // namespace lk
 
 using namespace lk;
 
+// Parts that a sequence's context is cut into, from the longest context that the
+// host expects (the blocks cut each sequence's own length).
+extern "C" int lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx) {
+  const int rows = Hq / Hkv * q_len, tiles = cdiv(rows, rows <= 8 ? 8 : 16);
+  const int64_t blocks = (int64_t)num_seqs * Hkv * tiles;
+  if (blocks == 0) return 1;
+  const int most = std::max(1, max_ctx / (PA_UNIT * PA_WARPS));  // a part has at least a unit per warp
+  const int64_t want = std::max<int64_t>(cdiv(4 * num_sms(), blocks), cdiv(max_ctx, 2048));
+  return (int)std::min<int64_t>(most, want);
+}
+
 extern "C" int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s) {
   LK_REQUIRE(d->Dh == 64 || d->Dh == 128, "page_attention: head_dim must be 64 or 128");
-  const int rows = d->num_seqs * d->q_len;
-  if (rows == 0) return 0;
-  const dim3 grid(rows, d->Hq);
-  if (d->kv_dtype == 1)
-    d->Dh == 64 ? page_attn_kernel<1, 64><<<grid, 128, 0, s>>>(*d) : page_attn_kernel<1, 128><<<grid, 128, 0, s>>>(*d);
-  else
-    d->Dh == 64 ? page_attn_kernel<2, 64><<<grid, 128, 0, s>>>(*d) : page_attn_kernel<2, 128><<<grid, 128, 0, s>>>(*d);
-  return check_launch("page_attention");
+  if (d->num_seqs == 0) return 0;
+  LK_REQUIRE(d->nsplit == 1 || (d->part_o && d->part_ml), "page_attention: split partial buffers needed");
+  const bool wide = d->Hq / d->Hkv * d->q_len > 8;
+#define LK_PA(KV, DH) return wide ? launch_page_attn<KV, DH, 2>(*d, s) : launch_page_attn<KV, DH, 1>(*d, s)
+  if (d->kv_dtype == 1) {
+    if (d->Dh == 64) LK_PA(1, 64);
+    LK_PA(1, 128);
+  }
+  if (d->Dh == 64) LK_PA(2, 64);
+  LK_PA(2, 128);
+#undef LK_PA
 }
