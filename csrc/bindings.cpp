@@ -1160,8 +1160,8 @@ int page_cache(const char* op, const torch::Tensor& k, const torch::Tensor& v, c
   TORCH_CHECK(k.is_contiguous(), op, ": k_cache must be contiguous");
   TORCH_CHECK(Hkv > 0 && page > 0 && (Dh == 64 || Dh == 128), op, ": head_dim must be 64 or 128");
   const int64_t slots = k.numel() / (Hkv * Dh);
-  TORCH_CHECK(k.numel() == v.numel() && slots * Hkv * Dh == k.numel() && slots % page == 0 && slots < (1ll << 31), op,
-              ": k_cache and v_cache are [pages * page, Hkv, Dh] of fewer than 2^31 slots");
+  TORCH_CHECK(k.numel() == v.numel() && slots * Hkv * Dh == k.numel() && slots > 0 && slots % page == 0 && slots < (1ll << 31), op,
+              ": k_cache and v_cache are [pages * page, Hkv, Dh], at least a page and fewer than 2^31 slots");
   TORCH_CHECK(ks.numel() == slots / page * Hkv && vs.numel() == ks.numel(), op, ": scales are [pages, Hkv]");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
               op, ": the cache must be 16-byte aligned");

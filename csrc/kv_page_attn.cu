@@ -21,10 +21,9 @@
 // 16-byte loads of the cached rows bring to each lane, the order of the
 // summed index being free (dims for K; a lane's dims are 16 neighbours of one
 // row).  tcgen05 would want both operands in 8 bits (the query rounded to them)
-// or the codes converted into shared memory first.  Each lane fills its own
-// slots of a ring with cp.async and reads them back itself: the asynchronous
-// copies need no barrier, and addresses are free, so any page size works and a
-// page may end inside a tile.
+// or the codes converted into shared memory first.  Each warp fills a ring of its
+// own with cp.async: no barrier between warps, and addresses are free, so any page
+// size works and a page may end inside a tile.
 //
 // Softmax per warp, one pass.  Weights are f16, so they are taken relative to
 // a running reference m with 2^7 at the largest one so far and moved only when
@@ -32,6 +31,8 @@
 // count.  A page's value scale 2^e enters as e added to the score, with a
 // reference of its own: a page of small values is then as exact as one of large
 // ones whichever the query looks at.  The softmax sum is kept in fp32 apart.
+#include <utility>
+
 #include "common.cuh"
 #include "host_util.h"
 #include "kv_page.cuh"
@@ -39,29 +40,59 @@
 
 namespace lk {
 
+#ifndef PA_STAGES
+#define PA_STAGES 2
+#endif
+#ifndef PA_BLOCKS
+#define PA_BLOCKS 3
+#endif
 constexpr int PA_WARPS = 4;
 constexpr int PA_UNIT = 32;        // tokens a warp takes at a time (two M = 16 tiles)
 constexpr float PA_LOW = -3.0e38f;  // reference before the first token
 constexpr float PA_TOP = 14.f, PA_AIM = 7.f;
 
+// A stage of a warp's ring: a unit's keys, values, scales and valid tokens.  Rows lie in
+// 128-byte lines (a line holds two tokens where DH = 64) whose 16-byte chunks are
+// exchanged by an XOR, so that the copies write whole lines and the fragment reads
+// touch every bank once: keys, 8 lanes read chunks 0-3 (or 4-7) of tokens 2a and
+// 2a + 1; values, 8 lanes read chunks 2b and 2b + 1 of tokens 0, 2, 4, 6 (or 1, 3, 5, 7)
+// of a group of 8, 16 lanes 32 bytes of each where DH = 64.
 template <int DH>
 struct PaRing {
-  static constexpr int KV_BYTES = PA_UNIT * DH;           // keys (or values) of a unit
-  static constexpr int SCALES = 2 * KV_BYTES;             // float2 (key, value scale) per token
-  static constexpr int MASK = SCALES + PA_UNIT * 8;       // bit per token: its page id is valid
-  static constexpr int STAGE = MASK + 16;
-  static constexpr int STAGES = 3;
+  static constexpr int KV_BYTES = PA_UNIT * DH;      // keys (or values) of a unit
+  static constexpr int SCALES = 2 * KV_BYTES;        // float2 (key, value scale) per token
+  static constexpr int MASK = SCALES + PA_UNIT * 8;  // bit per token: its page id is valid
+  static constexpr int STAGE = (MASK + 4 + 127) / 128 * 128;
+  static constexpr int STAGES = PA_STAGES;
   static constexpr int WARP = STAGE * STAGES;
+  // byte position of chunk k of token t
+  static __device__ __forceinline__ uint32_t at(int t, int k) {
+    if constexpr (DH == 128) return t * 128 + ((k ^ (t & 6) ^ ((t & 1) << 2)) << 4);
+    else return (t >> 1) * 128 + ((((t & 1) << 2 | k) ^ (t & 6)) << 4);
+  }
+  // the token of the unit that a lane copies a chunk of with its copy i
+  static constexpr int LANES = DH / 16;  // lanes per row
+  static __device__ __forceinline__ int token(int i, int lane) { return i * (32 / LANES) + lane / LANES; }
+  static __device__ __forceinline__ uint32_t place(int i, int lane) { return at(token(i, lane), lane % LANES); }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+// 16 bytes to shared address dst + OFF (a constant that stays in the instruction);
+// or zeros, with nothing read.
+template <int OFF>
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(on ? 8 : 0) : "memory");
+template <int OFF>
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16, %3;" ::"r"(dst), "l"(src), "n"(OFF), "r"(on ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_each(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>  // f(0), ..., f(N - 1), each argument a constant
+__device__ __forceinline__ void static_for(F f) {
+  static_for_each(f, std::make_integer_sequence<int, N>{});
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -88,8 +119,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 template <int KV, int HI>
 __device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
   if constexpr (KV == 1) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(HI ? w >> 16 : w & 0xFFFFu), __NV_E4M3);
-    return (uint32_t)h.x | (uint32_t)h.y << 16;
+    uint32_t h;
+    if constexpr (HI) asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi;\n}\n" : "=r"(h) : "r"(w));
+    else asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(h) : "r"(w));
+    return h;
   } else {
     const uint32_t u = __byte_perm(w ^ 0x80808080u, 0x64646464u, HI ? 0x4342 : 0x4140);
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
@@ -112,9 +145,18 @@ __device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int se
   return s;
 }
 
+// t / page = (t * magic) >> shift for 0 <= t < 2^31, with l = ceil(log2 page),
+// shift = 31 + l and magic = ceil(2^shift / page): magic * page exceeds 2^shift by less than
+// 2^l, so the product exceeds t 2^shift / page by less than 2^31 2^l / page = 2^shift / page.
+struct PaPlan {
+  int tiles, shift;
+  uint32_t magic;
+};
+
 // Grid: split fastest, then KV head, row tile (8 * NT query rows), sequence.
 template <int KV, int DH, int NT>
-__global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnDesc d, int tiles, int nsplit) {
+__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_attn_kernel(LkPageAttnDesc d, PaPlan plan) {
+  const int tiles = plan.tiles, nsplit = d.nsplit;
   using R = PaRing<DH>;
   constexpr int ROWS = 8 * NT, CH = DH / 64, MT = DH / 16;
   extern __shared__ __align__(16) uint8_t sm[];
@@ -131,63 +173,64 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
   const int u_end = min(sp.units, (split + 1) * sp.per);
   if (split > 0 && split * sp.per >= sp.units) return;
 
-  // this lane's tokens' addresses and this warp's ring
-  const int64_t tok_stride = (int64_t)d.Hkv * DH;
-  const uint8_t* kbase = (const uint8_t*)d.k_cache + h * DH;
-  const uint8_t* vbase = (const uint8_t*)d.v_cache + h * DH;
+  // where this lane copies from, and this warp's ring
+  const uint32_t tok_stride = (uint32_t)d.Hkv * DH;
+  const uint8_t* kbase = (const uint8_t*)d.k_cache + h * DH + lane % R::LANES * 16;
+  const uint8_t* vbase = (const uint8_t*)d.v_cache + h * DH + lane % R::LANES * 16;
   const int* table = d.tables + (int64_t)seq * d.max_pages;
   uint8_t* ring = sm + warp * R::WARP;
   const uint32_t ring_u = smem_u32(ring);
 
+  // t / page without a division: exact for 0 <= t < 2^31
+  auto page_index = [&](int t) { return (int)(((uint64_t)(uint32_t)t * plan.magic) >> plan.shift); };
   auto page_of = [&](int u) {
     const int t = u * PA_UNIT + lane;
-    return u < u_end && t < sp.end ? table[t / d.page] : 0;
+    return u < u_end && t < sp.end ? table[page_index(t)] : 0;
   };
-  auto issue = [&](int u, int stage, int pg) {
+  // the unit's copies: this lane looks up token `lane`, then copies 16 bytes of its share
+  // of the rows (8 lanes a 128-byte line, so that a request is a whole line); its token's
+  // scales go to registers and into the stage when the unit's turn comes
+  auto issue = [&](int u, int stage, int pg, float2& scales) {
     if (u < u_end) {
       const int t = u * PA_UNIT + lane;
-      bool ok = t < sp.end;
-      if (ok && (pg < 0 || pg >= d.num_pages)) {
-        if (d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-        ok = false;
-      }
-      const int slot = ok ? pg * d.page + t % d.page : -1;
-      const uint32_t st = ring_u + stage * R::STAGE;
+      const bool there = t < sp.end, ok = there && (unsigned)pg < (unsigned)d.num_pages;
       const unsigned valid = __ballot_sync(0xffffffffu, ok);
-      if (lane == 0) *reinterpret_cast<unsigned*>(ring + stage * R::STAGE + R::MASK) = valid;
+      const uint32_t st = ring_u + stage * R::STAGE;
+      const uint32_t slot = ok ? pg * d.page + (t - page_index(t) * d.page) : 0;
       const int64_t sc = ok ? (int64_t)pg * d.Hkv + h : 0;
-      cp_async4(st + R::SCALES + lane * 8, d.k_scale + sc, ok);
-      cp_async4(st + R::SCALES + lane * 8 + 4, d.v_scale + sc, ok);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // keys of tokens r, r + 8, r + 16, r + 24
-        const int s = __shfl_sync(0xffffffffu, slot, r + 8 * i);
-        const uint8_t* p = kbase + (s < 0 ? 0 : s) * tok_stride + c * 16;
-#pragma unroll
-        for (int k = 0; k < CH; ++k) cp_async16(st + ((i * CH + k) * 32 + lane) * 16, p + 64 * k, s >= 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {  // values of tokens 2c, 2c + 1, 2c + 8, 2c + 9, then 16 on
-        const int s = __shfl_sync(0xffffffffu, slot, 16 * (i >> 2) + 8 * ((i >> 1) & 1) + 2 * c + (i & 1));
-        const uint8_t* p = vbase + (s < 0 ? 0 : s) * tok_stride + r * (DH / 8);
-        if constexpr (DH == 128) cp_async16(st + R::KV_BYTES + (i * 32 + lane) * 16, p, s >= 0);
-        else cp_async8(st + R::KV_BYTES + (i * 32 + lane) * 8, p, s >= 0);
+      scales = make_float2(d.k_scale[sc], d.v_scale[sc]);
+      if (lane == 0) asm volatile("st.shared.u32 [%0+%1], %2;" ::"r"(st), "n"(R::MASK), "r"(valid) : "memory");
+      if (valid == 0xffffffffu) {
+        static_for<DH / 16>([&](auto i) {
+          const uint64_t off = (uint64_t)__shfl_sync(0xffffffffu, slot, R::token(i, lane)) * tok_stride;
+          cp_async16<0>(st + R::place(i, lane), kbase + off);
+          cp_async16<R::KV_BYTES>(st + R::place(i, lane), vbase + off);
+        });
+      } else {  // the end of the context, or a bad page id: nothing is read there, zeros take its place
+        if (there && !ok && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
+        static_for<DH / 16>([&](auto i) {
+          const uint64_t off = (uint64_t)__shfl_sync(0xffffffffu, slot, R::token(i, lane)) * tok_stride;
+          const bool on = (valid >> R::token(i, lane)) & 1;
+          cp_async16_or_zero<0>(st + R::place(i, lane), kbase + off, on);
+          cp_async16_or_zero<R::KV_BYTES>(st + R::place(i, lane), vbase + off, on);
+        });
       }
     }
     cp_commit();
   };
 
   // query fragments: column r of each tile, the dims of this lane's key bytes, times
-  // a power of two that brings the row's largest value to [2^7, 2^8) (f16 is then
-  // exact down to 2^-22 of it)
+  // a power of two that brings the tile's largest value to [2^14, 2^15): f16 then
+  // holds a bf16 value exactly down to 2^-31 of it, and 2^-39 of it is the rounding
   uint32_t qf[NT][4 * CH][2];
-  float qfac[NT][2];
   int lim[NT][2];
+  float amax = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int row = tile * ROWS + n * 8 + r;
-    uint32_t w[8 * CH];
+    uint32_t (&w)[4 * CH][2] = qf[n];  // bf16 pairs first
 #pragma unroll
-    for (int i = 0; i < 8 * CH; ++i) w[i] = 0;
+    for (int i = 0; i < 8 * CH; ++i) w[i / 2][i % 2] = 0;
     if (row < rows) {
       const uint4* p = reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.q +
                                                       ((int64_t)seq * d.q_len + row / group) * d.ldq +
@@ -197,32 +240,31 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint4 v = p[k * 8 + c * 2 + i];
-          w[k * 8 + i * 4] = v.x, w[k * 8 + i * 4 + 1] = v.y, w[k * 8 + i * 4 + 2] = v.z, w[k * 8 + i * 4 + 3] = v.w;
+          w[k * 4 + i * 2][0] = v.x, w[k * 4 + i * 2][1] = v.y, w[k * 4 + i * 2 + 1][0] = v.z, w[k * 4 + i * 2 + 1][1] = v.w;
         }
     }
-    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8 * CH; ++i) {
-      const float2 f = unpack_bf16x2(w[i]);
+      const float2 f = unpack_bf16x2(w[i / 2][i % 2]);
       if (fabsf(f.x) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.x));
       if (fabsf(f.y) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.y));
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -119);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+  }
+  const int e = max((int)(__float_as_uint(warp_max(amax)) >> 23) - 127 - 14, -112);
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+  const float qfac = __uint_as_float((uint32_t)(127 + e) << 23) * (d.scale * 1.4426950408889634f);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int k = 0; k < 4 * CH; ++k)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float2 f = unpack_bf16x2(w[2 * k + i]);
+        const float2 f = unpack_bf16x2(qf[n][k][i]);
         const __half2 hv = __floats2half2_rn(f.x * down, f.y * down);
         qf[n][k][i] = *reinterpret_cast<const uint32_t*>(&hv);
       }
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23) * (d.scale * 1.4426950408889634f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      qfac[n][i] = __shfl_sync(0xffffffffu, up, (2 * c + i) * 4);
       const int col = tile * ROWS + n * 8 + 2 * c + i;
       lim[n][i] = col < rows ? sp.ctx - d.q_len + col / group + 1 : sp.end;
     }
@@ -241,14 +283,16 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
   }
 
   int u = split * sp.per + warp;
+  float2 scales[R::STAGES];  // of the units in flight, the next one first
 #pragma unroll
-  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, page_of(u + s * PA_WARPS));
+  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, page_of(u + s * PA_WARPS), scales[s]);
   int pg = page_of(u + R::STAGES * PA_WARPS);
   int stage = 0;
   for (; u < u_end; u += PA_WARPS) {
+    uint8_t* st = ring + stage * R::STAGE;
+    *reinterpret_cast<float2*>(st + R::SCALES + lane * 8) = scales[0];
     cp_wait<R::STAGES - 1>();
     __syncwarp();
-    const uint8_t* st = ring + stage * R::STAGE;
     // scores of both 16-token tiles
     float s[2][NT][4];
 #pragma unroll
@@ -259,9 +303,9 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
         for (int i = 0; i < 4; ++i) s[g][n][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
-        const uint4 x = *reinterpret_cast<const uint4*>(st + ((2 * g * CH + k) * 32 + lane) * 16);
-        const uint4 y = *reinterpret_cast<const uint4*>(st + (((2 * g + 1) * CH + k) * 32 + lane) * 16);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const uint4 lo = *reinterpret_cast<const uint4*>(st + R::at(16 * g + r, 4 * k + c));
+        const uint4 hi = *reinterpret_cast<const uint4*>(st + R::at(16 * g + r + 8, 4 * k + c));
+        const uint32_t xs[4] = {lo.x, lo.y, lo.z, lo.w}, ys[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t a0 = codes_f16x2<KV, 0>(xs[i]), a1 = codes_f16x2<KV, 0>(ys[i]);
@@ -272,40 +316,51 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
       }
     }
     // scale, mask; the score plus the value scale's exponent is the weight's exponent
-    const unsigned valid = *reinterpret_cast<const unsigned*>(st + R::MASK);
-    const bool all = valid == 0xffffffffu && (u + 1) * PA_UNIT <= open;
-    float lv[2][2];
-    bool move = false;
+    float x[2][NT][4];
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int tl = 16 * g + 8 * i + r;
-        const float2 sc = *reinterpret_cast<const float2*>(st + R::SCALES + tl * 8);
-        lv[g][i] = __log2f(sc.y);
+        const float2 sc = *reinterpret_cast<const float2*>(st + R::SCALES + (16 * g + 8 * i + r) * 8);
+        const float kf = sc.x * qfac, lv = __log2f(sc.y);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            float x = s[g][n][2 * i + q] * sc.x * qfac[n][q];
-            if (!all && (u * PA_UNIT + tl >= lim[n][q] || !((valid >> tl) & 1))) x = -INFINITY;
-            s[g][n][2 * i + q] = x;
-            move |= x > ms[n][q] + PA_TOP || x + lv[g][i] > mw[n][q] + PA_TOP;
+            s[g][n][2 * i + q] *= kf;
+            x[g][n][2 * i + q] = s[g][n][2 * i + q] + lv;
           }
+      }
+    const unsigned valid = *reinterpret_cast<const unsigned*>(st + R::MASK);
+    if (valid != 0xffffffffu || (u + 1) * PA_UNIT > open) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int tl = 16 * g + 8 * i + r;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              if (u * PA_UNIT + tl >= lim[n][q] || !((valid >> tl) & 1)) s[g][n][2 * i + q] = x[g][n][2 * i + q] = -INFINITY;
+        }
+    }
+    float sa[NT][2], xa[NT][2];
+    bool move = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        sa[n][q] = fmaxf(fmaxf(s[0][n][q], s[0][n][2 + q]), fmaxf(s[1][n][q], s[1][n][2 + q]));
+        xa[n][q] = fmaxf(fmaxf(x[0][n][q], x[0][n][2 + q]), fmaxf(x[1][n][q], x[1][n][2 + q]));
+        move |= sa[n][q] > ms[n][q] + PA_TOP || xa[n][q] > mw[n][q] + PA_TOP;
       }
     if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          float a = -INFINITY, w = -INFINITY;
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              a = fmaxf(a, s[g][n][2 * i + q]);
-              w = fmaxf(w, s[g][n][2 * i + q] + lv[g][i]);
-            }
+          float a = sa[n][q], w = xa[n][q];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
@@ -335,9 +390,8 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
           float w[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const float x = s[g][n][2 * i + q];
-            l[n][q] += fast_exp2(x - ms[n][q]);
-            w[q] = fast_exp2(x + lv[g][i] - mw[n][q]);
+            l[n][q] += fast_exp2(s[g][n][2 * i + q] - ms[n][q]);
+            w[q] = fast_exp2(x[g][n][2 * i + q] - mw[n][q]);
           }
           const __half2 hv = __floats2half2_rn(w[0], w[1]);
           p[g][n][i] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
@@ -348,11 +402,12 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
       uint32_t v[4][DH / 32];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const int tok = 16 * g + 8 * (i >> 1) + 2 * c + (i & 1);
         if constexpr (DH == 128) {
-          const uint4 x = *reinterpret_cast<const uint4*>(st + R::KV_BYTES + ((4 * g + i) * 32 + lane) * 16);
+          const uint4 x = *reinterpret_cast<const uint4*>(st + R::KV_BYTES + R::at(tok, r));
           v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
         } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(st + R::KV_BYTES + ((4 * g + i) * 32 + lane) * 8);
+          const uint2 x = *reinterpret_cast<const uint2*>(st + R::KV_BYTES + R::at(tok, r >> 1) + (r & 1) * 8);
           v[i][0] = x.x, v[i][1] = x.y;
         }
       }
@@ -368,8 +423,10 @@ __global__ void __launch_bounds__(32 * PA_WARPS, 2) page_attn_kernel(LkPageAttnD
           for (int n = 0; n < NT; ++n) mma_f16(acc[n][2 * m + o], a0, a1, a2, a3, p[g][n][0], p[g][n][1]);
         }
     }
-    __syncwarp();  // every lane is done with the stage's scales and mask
-    issue(u + R::STAGES * PA_WARPS, stage, pg);
+    __syncwarp();  // every lane is done with the stage
+#pragma unroll
+    for (int i = 0; i + 1 < R::STAGES; ++i) scales[i] = scales[i + 1];
+    issue(u + R::STAGES * PA_WARPS, stage, pg, scales[R::STAGES - 1]);
     pg = page_of(u + (R::STAGES + 1) * PA_WARPS);
     stage = stage + 1 == R::STAGES ? 0 : stage + 1;
   }
@@ -466,7 +523,10 @@ static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
   constexpr int smem = ring > merge ? ring : merge;
   auto k = page_attn_kernel<KV, DH, NT>;
   cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, tiles, d.nsplit);
+  PaPlan plan{tiles, 31, 0};
+  while ((1ll << (plan.shift - 31)) < d.page) ++plan.shift;
+  plan.magic = (uint32_t)(((1ull << plan.shift) + d.page - 1) / d.page);
+  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, plan);
   if (check_launch("page_attention")) return -1;
   if (d.nsplit == 1) return 0;
   const int64_t warps = (int64_t)d.num_seqs * d.q_len * d.Hq;
