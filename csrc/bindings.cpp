@@ -1251,7 +1251,7 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
   d.status = status.data_ptr<int>();
   if (max_ctx <= 0 || max_ctx > tables.size(1) * page) max_ctx = tables.size(1) * page;
   TORCH_CHECK(max_ctx < (1ll << 31) - 64, "page_attention: contexts of fewer than 2^31 tokens");
-  d.nsplit = lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)max_ctx);
+  lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)max_ctx, &d.nsplit, &d.min_units);
   torch::Tensor part;  // allocated per call: the allocator knows the stream
   if (d.nsplit > 1) {
     const int64_t parts = q.size(0) * Hq * d.nsplit;

@@ -131,17 +131,17 @@ __device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
 }
 
 // What the blocks of a sequence's row tile share: the tokens [0, end) that any of
-// its queries sees, cut into nsplit parts of `per` units.
+// its queries sees, cut into at most nsplit parts of `per` units.
 struct PaSpan {
   int ctx, end, units, per;
 };
 
-__device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int seq, int last_row, int group, int nsplit) {
+__device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int seq, int last_row, int group) {
   PaSpan s;
   s.ctx = (int)min((int64_t)max(d.ctx_lens[seq], 0), (int64_t)d.max_pages * d.page);
   s.end = max(0, s.ctx - d.q_len + last_row / group + 1);
   s.units = (s.end + PA_UNIT - 1) / PA_UNIT;
-  s.per = max((s.units + nsplit - 1) / nsplit, PA_WARPS);
+  s.per = max((s.units + d.nsplit - 1) / d.nsplit, d.min_units);
   return s;
 }
 
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
   const int tile = b % tiles, seq = b / tiles;
   const int group = d.Hq / d.Hkv, rows = group * d.q_len;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const PaSpan sp = page_attn_span(d, seq, min(rows, (tile + 1) * ROWS) - 1, group, nsplit);
+  const PaSpan sp = page_attn_span(d, seq, min(rows, (tile + 1) * ROWS) - 1, group);
   if (threadIdx.x == 0 && d.ctx_lens[seq] > (int64_t)d.max_pages * d.page && d.status)
     atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
   const int u_end = min(sp.units, (split + 1) * sp.per);
@@ -218,6 +218,12 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
     }
     cp_commit();
   };
+
+  int u = split * sp.per + warp;
+  float2 scales[R::STAGES];  // of the units in flight, the next one first
+#pragma unroll
+  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, page_of(u + s * PA_WARPS), scales[s]);
+  int pg = page_of(u + R::STAGES * PA_WARPS);
 
   // query fragments: column r of each tile, the dims of this lane's key bytes, times
   // a power of two that brings the tile's largest value to [2^14, 2^15): f16 then
@@ -282,11 +288,6 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
     for (int i = 0; i < 2; ++i) ms[n][i] = mw[n][i] = PA_LOW, l[n][i] = 0.f;
   }
 
-  int u = split * sp.per + warp;
-  float2 scales[R::STAGES];  // of the units in flight, the next one first
-#pragma unroll
-  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, page_of(u + s * PA_WARPS), scales[s]);
-  int pg = page_of(u + R::STAGES * PA_WARPS);
   int stage = 0;
   for (; u < u_end; u += PA_WARPS) {
     uint8_t* st = ring + stage * R::STAGE;
@@ -491,7 +492,7 @@ __global__ void page_attn_join_kernel(LkPageAttnDesc d, int tile_rows, int nspli
   const int head = (int)(w % d.Hq), group = d.Hq / d.Hkv;
   const int row = (int)(grow % d.q_len) * group + head % group;
   const int last = min(group * d.q_len, (row / tile_rows + 1) * tile_rows) - 1;
-  const PaSpan sp = page_attn_span(d, (int)(grow / d.q_len), last, group, nsplit);
+  const PaSpan sp = page_attn_span(d, (int)(grow / d.q_len), last, group);
   const int used = max(1, (sp.units + sp.per - 1) / sp.per);
   const float4* ml = reinterpret_cast<const float4*>(d.part_ml) + w * nsplit;
   float MS = PA_LOW, MW = PA_LOW, L = 0.f, o[DH / 32];
@@ -538,15 +539,17 @@ static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
 
 using namespace lk;
 
-// Parts that a sequence's context is cut into, from the longest context that the
-// host expects (the blocks cut each sequence's own length).
-extern "C" int lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx) {
-  const int rows = Hq / Hkv * q_len, tiles = cdiv(rows, rows <= 8 ? 8 : 16);
-  const int64_t blocks = (int64_t)num_seqs * Hkv * tiles;
-  if (blocks == 0) return 1;
-  const int most = std::max(1, max_ctx / (PA_UNIT * PA_WARPS));  // a part has at least a unit per warp
-  const int64_t want = std::max<int64_t>(cdiv(4 * num_sms(), blocks), cdiv(max_ctx, 2048));
-  return (int)std::min<int64_t>(most, want);
+// Into how many parts a context may be cut, and the least units of a part, from the
+// longest context that the host expects (each block cuts its sequence's own length).
+// A block costs what 150 tokens cost beside its part (2.3 us), so parts are as few as
+// fill the GPU: 2.5 blocks an SM (1 reaches 60 % of the rate of 2 or 3), of 256 tokens
+// at least.  Where the sequences alone fill it, only contexts over 4096 are cut, so
+// that one of them does not run on alone.
+extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units) {
+  const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
+  const int fill = (int)std::max<int64_t>(1, 5 * num_sms() / 2 / blocks), length = cdiv(max_ctx, 4096);
+  *nsplit = std::max(1, std::min(std::max(fill, length), cdiv(max_ctx, 256)));
+  *min_units = fill > 1 ? 256 / PA_UNIT : 4096 / PA_UNIT;
 }
 
 extern "C" int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s) {
