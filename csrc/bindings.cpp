@@ -1180,6 +1180,8 @@ void page_append(torch::Tensor qkv, int64_t Hq, int64_t Hkv, int64_t Dh, torch::
   need(qkv, "qkv", torch::kBFloat16);
   TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && Hq >= 0 && qkv.size(1) == (Hq + 2 * Hkv) * Dh,
               "page_append: qkv must be row-major [T, (Hq + 2 Hkv) * Dh]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0 && (qkv.stride(0) % 8 == 0 || qkv.size(0) <= 1),
+              "page_append: the rows of qkv must be 16-byte aligned");
   need_contig(slots, "slots", torch::kInt32);
   TORCH_CHECK(slots.numel() == qkv.size(0), "page_append: one slot per row");
   LkPageAppendDesc d{};
@@ -1202,6 +1204,8 @@ void page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_s
   need(out, "out", torch::kBFloat16);
   TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == slots.numel() && out.size(1) == 2 * Hkv * Dh,
               "page_gather: out must be row-major [n, 2 * Hkv * Dh]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0 && (out.stride(0) % 8 == 0 || out.size(0) <= 1),
+              "page_gather: the rows of out must be 16-byte aligned");
   LkPageGatherDesc d{};
   d.kv_dtype = page_cache("page_gather", k_cache, v_cache, k_scale, v_scale, Hkv, Dh, page);
   same_device("page_gather", out, {&slots, &k_cache, &v_cache, &k_scale, &v_scale, &status});

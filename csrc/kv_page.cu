@@ -21,83 +21,193 @@
 namespace lk {
 
 // ---------------------------------------------------------------- append
-// Row t starts a run when it does not continue row t - 1 inside one page.
-__device__ __forceinline__ bool starts_run(const int* slots, int t, int page) {
-  const int s = slots[t];
-  return t == 0 || slots[t - 1] < 0 || s != slots[t - 1] + 1 || s % page == 0;
+// A run is the rows of a call that go to one page: consecutive rows with
+// consecutive slots.  One warp takes a run's keys or values of one head: 16 bytes
+// (8 dims) a lane, RPI rows at a time, the first 8 of those steps kept in registers
+// between the pass for the maximum and the pass that encodes, which is all of a page
+// of 16 rows (32 at head_dim 64); longer runs read the rest again, from L1 or L2.
+//
+// Bound by HBM for a prompt (6 bytes a value with the codes written: 8190 rows of 8
+// heads x 128 in 14 us), by the chain slot -> row -> maximum -> store for a token
+// per sequence.  A block's warps look for runs that start in its `window` rows: 1 row
+// where there are few (every run on a block of its own), 8 for prompts, where
+// 15 of 16 rows start none and their blocks would be empty.
+
+// 8 bf16 -> 8 codes.  CHECK: some of them are not finite (infinities saturate, NaN -> 0).
+template <int KV, bool CHECK>
+__device__ __forceinline__ uint2 encode8(uint4 x, float inv) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t out[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f = unpack_bf16x2(w[i]);
+    f.x *= inv, f.y *= inv;
+    uint32_t two;
+    if constexpr (CHECK) two = page_encode<KV>(f.x) | page_encode<KV>(f.y) << 8;
+    else if constexpr (KV == 1) two = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    else two = (__float2int_rn(f.x) & 0xFF) | (__float2int_rn(f.y) & 0xFF) << 8;
+    out[i / 2] |= two << (16 * (i & 1));
+  }
+  return make_uint2(out[0], out[1]);
 }
 
-// One warp per (row, KV head, K|V); the warps of rows that start a run (the new
-// rows of one page) do the run's work: amax, the page's new scale, the codes
-// already in the page moved to it when it grew, the new codes.
-template <int KV, int DH>
-__global__ void page_append_kernel(LkPageAppendDesc d) {
-  constexpr int PER = DH / 32;
-  const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= (int64_t)d.T * d.Hkv * 2) return;
-  const int which = (int)(w & 1);
-  const int h = (int)((w >> 1) % d.Hkv);
-  const int t = (int)((w >> 1) / d.Hkv);
-  const int slot = d.slots[t];
-  if (slot < 0 || !starts_run(d.slots, t, d.page)) return;
-  if (slot >= d.num_slots) {
-    if (lane == 0 && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-    return;
+// 8 codes moved to a larger scale (f = old / new <= 1): always finite.
+template <int KV>
+__device__ __forceinline__ uint2 move8(uint2 c, float f) {
+  uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out |= (uint32_t)page_encode<KV>(page_decode<KV>((uint8_t)(w[i] >> (8 * k))) * f) << (8 * k);
+    w[i] = out;
   }
-  const int pg = slot / d.page, first = slot % d.page;
-  int rows = 1;
-  while (t + rows < d.T && first + rows < d.page && d.slots[t + rows] == slot + rows) ++rows;
-  const __nv_bfloat16* src = (const __nv_bfloat16*)d.qkv + (int64_t)t * d.ld + (d.Hq + which * d.Hkv + h) * DH;
-  uint8_t* codes = (uint8_t*)(which ? d.v_cache : d.k_cache);
-  float* scale = (which ? d.v_scale : d.k_scale) + (int64_t)pg * d.Hkv + h;
-  float amax = 0.f;
-  for (int r = 0; r < rows; ++r)
-    for (int i = 0; i < PER; ++i) {
-      const float a = fabsf(__bfloat162float(src[r * d.ld + i * 32 + lane]));
-      if (a <= 3.4028234e38f) amax = fmaxf(amax, a);  // neither inf nor NaN
-    }
-  float now = page_scale<KV>(warp_max(amax));
-  if (first > 0) {
-    const float old = *scale;
-    now = fmaxf(now, old);
-    if (now > old) {
-      const float f = old / now;
-      for (int r = 0; r < first; ++r)
-        for (int i = 0; i < PER; ++i) {
-          uint8_t* c = codes + ((int64_t)(pg * (int64_t)d.page + r) * d.Hkv + h) * DH + i * 32 + lane;
-          *c = page_encode<KV>(page_decode<KV>(*c) * f);
-        }
+  return make_uint2(w[0], w[1]);
+}
+
+// largest |x| bits of 8 bf16, as the larger of two 16-bit halves
+__device__ __forceinline__ uint32_t top8(uint32_t top, uint4 x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+  return top;
+}
+
+template <int KV, int DH>
+__device__ void append_run(const LkPageAppendDesc& d, int t, int rows, int slot, int h, bool value) {
+  constexpr int LPR = DH / 8, RPI = 32 / LPR, HELD = 8;
+  const int lane = threadIdx.x & 31, sub = lane / LPR, col = lane % LPR * 8;
+  const int64_t pg = slot / d.page;
+  const int first = slot - (int)pg * d.page;
+  const __nv_bfloat16* src =
+      (const __nv_bfloat16*)d.qkv + (int64_t)t * d.ld + (d.Hq + (value ? d.Hkv : 0) + h) * DH + col;
+  const int64_t pitch = (int64_t)d.Hkv * DH;
+  uint8_t* dst = (uint8_t*)(value ? d.v_cache : d.k_cache) + slot * pitch + h * DH + col;
+  float* scale = (value ? d.v_scale : d.k_scale) + pg * d.Hkv + h;
+  const float old = first > 0 ? *scale : 0.f;
+  uint4 x[HELD];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int r = i * RPI + sub;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (r < rows) x[i] = *reinterpret_cast<const uint4*>(src + r * d.ld);
+  }
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) top = top8(top, x[i]);
+  for (int r = HELD * RPI + sub; r < rows; r += RPI) top = top8(top, *reinterpret_cast<const uint4*>(src + r * d.ld));
+  top = max(top & 0xFFFFu, top >> 16);
+  const bool special = __any_sync(0xffffffffu, top >= 0x7F80u);  // infinities or NaN among them
+  if (special) {  // the maximum of the finite ones
+    top = 0;
+    for (int r = sub; r < rows; r += RPI)
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = __bfloat16_as_ushort(src[r * d.ld + i]) & 0x7FFFu;
+        if (a < 0x7F80u) top = max(top, a);
+      }
+  }
+  float now = page_scale<KV>(__uint_as_float(__reduce_max_sync(0xffffffffu, top) << 16));
+  if (first > 0 && old >= now) now = old;
+  else if (first > 0) {  // the rows already there move to the new scale
+    const float f = old / now;
+    for (int r = sub; r < first; r += RPI) {
+      uint2* c = reinterpret_cast<uint2*>(dst + (r - first) * pitch);
+      *c = move8<KV>(*c, f);
     }
   }
   const float inv = 1.f / now;
-  for (int r = 0; r < rows; ++r)
-    for (int i = 0; i < PER; ++i)
-      codes[((int64_t)(slot + r) * d.Hkv + h) * DH + i * 32 + lane] =
-          page_encode<KV>(__bfloat162float(src[r * d.ld + i * 32 + lane]) * inv);
-  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int r = i * RPI + sub;
+    if (r < rows) *reinterpret_cast<uint2*>(dst + r * pitch) = special ? encode8<KV, true>(x[i], inv) : encode8<KV, false>(x[i], inv);
+  }
+  for (int r = HELD * RPI + sub; r < rows; r += RPI) {
+    const uint4 y = *reinterpret_cast<const uint4*>(src + r * d.ld);
+    *reinterpret_cast<uint2*>(dst + r * pitch) = special ? encode8<KV, true>(y, inv) : encode8<KV, false>(y, inv);
+  }
   if (lane == 0) *scale = now;
 }
 
-// ---------------------------------------------------------------- gather
-template <int KV>
-__global__ void page_gather_kernel(LkPageGatherDesc d) {
-  const int64_t total = (int64_t)d.n * 2 * d.Hkv * d.Dh;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int c = (int)(i % d.Dh);
-    const int64_t r = i / d.Dh;
-    const int h = (int)(r % d.Hkv), which = (int)((r / d.Hkv) & 1), t = (int)(r / (2 * d.Hkv));
-    const int slot = d.slots[t];
-    float v = 0.f;
-    if (slot < 0 || slot >= d.num_slots) {
-      if (d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-    } else {
-      const uint8_t* codes = (const uint8_t*)(which ? d.v_cache : d.k_cache);
-      v = page_decode<KV>(codes[((int64_t)slot * d.Hkv + h) * d.Dh + c]) *
-          (which ? d.v_scale : d.k_scale)[(int64_t)(slot / d.page) * d.Hkv + h];
+// grid (windows of rows, groups of 8 (head, K|V) pairs)
+template <int KV, int DH>
+__global__ void __launch_bounds__(256) page_append_kernel(LkPageAppendDesc d, int window) {
+  const int item = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (item >= 2 * d.Hkv) return;
+  // lane l looks at row t0 - 1 + l: which rows continue the row before them
+  const int t0 = blockIdx.x * window, t = t0 - 1 + lane;
+  const int s = t >= 0 && t < d.T ? d.slots[t] : -1;
+  const int before = __shfl_up_sync(0xffffffffu, s, 1);
+  const bool more = lane > 0 && s > 0 && before >= 0 && s == before + 1 && s % d.page != 0;
+  const unsigned goes_on = __ballot_sync(0xffffffffu, more);
+  unsigned starts = __ballot_sync(0xffffffffu, lane > 0 && lane <= window && s >= 0 && !more);
+  while (starts) {
+    const int l = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const int slot = __shfl_sync(0xffffffffu, s, l);
+    if (slot >= d.num_slots) {
+      if (lane == 0 && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
+      continue;
     }
-    ((__nv_bfloat16*)d.out)[(int64_t)t * d.ldo + (which * d.Hkv + h) * d.Dh + c] = __float2bfloat16(v);
+    const unsigned rest = l == 31 ? 0u : goes_on >> (l + 1);
+    int rows = 1 + __ffs(~rest) - 1;  // rest has a zero: its top bit
+    if (l + rows == 32) {             // as far as this warp looked: on from there
+      const int room = d.page - slot % d.page;
+      for (bool all = true; all;) {
+        const int tr = t0 - 1 + l + rows + lane;
+        const bool here = rows + lane < room && tr < d.T && d.slots[tr] == slot + rows + lane;
+        const unsigned m = __ballot_sync(0xffffffffu, here);
+        all = m == 0xffffffffu;
+        rows += all ? 32 : __ffs(~m) - 1;
+      }
+    }
+    append_run<KV, DH>(d, t0 - 1 + l, rows, slot, item >> 1, item & 1);
   }
+}
+
+// ---------------------------------------------------------------- gather
+// A thread takes 16 codes of a token's keys and the same 16 of its values (the heads
+// of a slot lie side by side in the cache and in the output alike): two 16-byte loads,
+// 32 + 32 bytes written.  Bound by HBM: 3 bytes a value.
+template <int KV>
+__device__ __forceinline__ void widen16(const uint8_t* src, float scale, __nv_bfloat16* dst) {
+  const uint4 c = *reinterpret_cast<const uint4*>(src);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a, b;
+    const uint32_t two = w[i / 2] >> (16 * (i & 1));
+    if constexpr (KV == 1) {
+      const __half2_raw h2 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xFFFFu), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+      a = f.x, b = f.y;
+    } else {
+      a = (float)(int8_t)(two & 0xFFu), b = (float)(int8_t)(two >> 8 & 0xFFu);
+    }
+    o[i] = pack_bf16x2(a * scale, b * scale);
+  }
+  reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+template <int KV>
+__global__ void __launch_bounds__(256) page_gather_kernel(LkPageGatherDesc d, int total, FastDiv per_row, FastDiv page) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int t = per_row.div(i), at = (i - t * per_row.d) * 16;
+  const int h = at / d.Dh, width = d.Hkv * d.Dh;
+  const int slot = d.slots[t];
+  __nv_bfloat16* out = (__nv_bfloat16*)d.out + (int64_t)t * d.ldo + at;
+  if (slot < 0 || slot >= d.num_slots) {
+    if (d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
+    const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) reinterpret_cast<uint4*>(out)[k] = z, reinterpret_cast<uint4*>(out + width)[k] = z;
+    return;
+  }
+  const int64_t sc = (int64_t)page.div(slot) * d.Hkv + h, from = (int64_t)slot * width + at;
+  widen16<KV>((const uint8_t*)d.k_cache + from, d.k_scale[sc], out);
+  widen16<KV>((const uint8_t*)d.v_cache + from, d.v_scale[sc], out + width);
 }
 
 // ---------------------------------------------------------------- page copies
@@ -130,21 +240,27 @@ using namespace lk;
 
 extern "C" int lk_page_append(const LkPageAppendDesc* d, cudaStream_t s) {
   LK_REQUIRE(d->Dh == 64 || d->Dh == 128, "page_append: head_dim must be 64 or 128");
-  const int64_t warps = (int64_t)d->T * d->Hkv * 2;
-  if (warps == 0) return 0;
-  const int grid = cdiv(warps * 32, 256);
+  if (d->T == 0 || d->Hkv == 0) return 0;
+  LK_REQUIRE(d->Hkv <= 4 * 65535, "page_append: too many heads");
+  const int window = d->T <= 1024 ? 1 : 8;
+  const dim3 grid(cdiv(d->T, window), cdiv(2 * d->Hkv, 8));
   if (d->kv_dtype == 1)
-    d->Dh == 64 ? page_append_kernel<1, 64><<<grid, 256, 0, s>>>(*d) : page_append_kernel<1, 128><<<grid, 256, 0, s>>>(*d);
+    d->Dh == 64 ? page_append_kernel<1, 64><<<grid, 256, 0, s>>>(*d, window) : page_append_kernel<1, 128><<<grid, 256, 0, s>>>(*d, window);
   else
-    d->Dh == 64 ? page_append_kernel<2, 64><<<grid, 256, 0, s>>>(*d) : page_append_kernel<2, 128><<<grid, 256, 0, s>>>(*d);
+    d->Dh == 64 ? page_append_kernel<2, 64><<<grid, 256, 0, s>>>(*d, window) : page_append_kernel<2, 128><<<grid, 256, 0, s>>>(*d, window);
   return check_launch("page_append");
 }
 
 extern "C" int lk_page_gather(const LkPageGatherDesc* d, cudaStream_t s) {
-  const int64_t work = (int64_t)d->n * 2 * d->Hkv * d->Dh;
-  if (work == 0) return 0;
-  const int grid = (int)std::min<int64_t>((work + 255) / 256, (int64_t)num_sms() * 8);
-  d->kv_dtype == 1 ? page_gather_kernel<1><<<grid, 256, 0, s>>>(*d) : page_gather_kernel<2><<<grid, 256, 0, s>>>(*d);
+  const int per_row = d->Hkv * d->Dh / 16;
+  const int64_t total = (int64_t)d->n * per_row;
+  if (total == 0) return 0;
+  LK_REQUIRE(total < (1ll << 31), "page_gather: too many rows in one call");
+  const int grid = cdiv(total, 256);
+  if (d->kv_dtype == 1)
+    page_gather_kernel<1><<<grid, 256, 0, s>>>(*d, (int)total, FastDiv(per_row), FastDiv(d->page));
+  else
+    page_gather_kernel<2><<<grid, 256, 0, s>>>(*d, (int)total, FastDiv(per_row), FastDiv(d->page));
   return check_launch("page_gather");
 }
 

@@ -40,4 +40,17 @@ __device__ __forceinline__ float page_decode(uint8_t c) {
   else return (float)(int8_t)c;
 }
 
+// n / d = (n * magic) >> shift for 0 <= n < 2^31, with l = ceil(log2 d), shift = 31 + l
+// and magic = ceil(2^shift / d): magic * d exceeds 2^shift by less than 2^l, so the product
+// exceeds n 2^shift / d by less than 2^31 2^l / d = 2^shift / d.
+struct FastDiv {
+  uint32_t magic;
+  int shift, d;
+  explicit FastDiv(int divisor) : magic(0), shift(31), d(divisor) {
+    while ((1ll << (shift - 31)) < divisor) ++shift;
+    magic = (uint32_t)(((1ull << shift) + divisor - 1) / divisor);
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * magic) >> shift); }
+};
+
 }  // namespace lk

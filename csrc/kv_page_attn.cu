@@ -31,6 +31,7 @@
 // count.  A page's value scale 2^e enters as e added to the score, with a
 // reference of its own: a page of small values is then as exact as one of large
 // ones whichever the query looks at.  The softmax sum is kept in fp32 apart.
+#include <algorithm>
 #include <utility>
 
 #include "common.cuh"
@@ -145,18 +146,10 @@ __device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int se
   return s;
 }
 
-// t / page = (t * magic) >> shift for 0 <= t < 2^31, with l = ceil(log2 page),
-// shift = 31 + l and magic = ceil(2^shift / page): magic * page exceeds 2^shift by less than
-// 2^l, so the product exceeds t 2^shift / page by less than 2^31 2^l / page = 2^shift / page.
-struct PaPlan {
-  int tiles, shift;
-  uint32_t magic;
-};
-
 // Grid: split fastest, then KV head, row tile (8 * NT query rows), sequence.
 template <int KV, int DH, int NT>
-__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_attn_kernel(LkPageAttnDesc d, PaPlan plan) {
-  const int tiles = plan.tiles, nsplit = d.nsplit;
+__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_attn_kernel(LkPageAttnDesc d, int tiles, FastDiv pages) {
+  const int nsplit = d.nsplit;
   using R = PaRing<DH>;
   constexpr int ROWS = 8 * NT, CH = DH / 64, MT = DH / 16;
   extern __shared__ __align__(16) uint8_t sm[];
@@ -171,6 +164,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
   if (threadIdx.x == 0 && d.ctx_lens[seq] > (int64_t)d.max_pages * d.page && d.status)
     atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
   const int u_end = min(sp.units, (split + 1) * sp.per);
+  cudaTriggerProgrammaticLaunchCompletion();  // the join may be brought up; it waits for all of this grid
   if (split > 0 && split * sp.per >= sp.units) return;
 
   // where this lane copies from, and this warp's ring
@@ -181,11 +175,9 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
   uint8_t* ring = sm + warp * R::WARP;
   const uint32_t ring_u = smem_u32(ring);
 
-  // t / page without a division: exact for 0 <= t < 2^31
-  auto page_index = [&](int t) { return (int)(((uint64_t)(uint32_t)t * plan.magic) >> plan.shift); };
   auto page_of = [&](int u) {
     const int t = u * PA_UNIT + lane;
-    return u < u_end && t < sp.end ? table[page_index(t)] : 0;
+    return u < u_end && t < sp.end ? table[pages.div(t)] : 0;
   };
   // the unit's copies: this lane looks up token `lane`, then copies 16 bytes of its share
   // of the rows (8 lanes a 128-byte line, so that a request is a whole line); its token's
@@ -196,7 +188,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
       const bool there = t < sp.end, ok = there && (unsigned)pg < (unsigned)d.num_pages;
       const unsigned valid = __ballot_sync(0xffffffffu, ok);
       const uint32_t st = ring_u + stage * R::STAGE;
-      const uint32_t slot = ok ? pg * d.page + (t - page_index(t) * d.page) : 0;
+      const uint32_t slot = ok ? pg * d.page + (t - pages.div(t) * d.page) : 0;
       const int64_t sc = ok ? (int64_t)pg * d.Hkv + h : 0;
       scales = make_float2(d.k_scale[sc], d.v_scale[sc]);
       if (lane == 0) asm volatile("st.shared.u32 [%0+%1], %2;" ::"r"(st), "n"(R::MASK), "r"(valid) : "memory");
@@ -487,6 +479,7 @@ template <int DH>
 __global__ void page_attn_join_kernel(LkPageAttnDesc d, int tile_rows, int nsplit) {
   const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
+  cudaGridDependencySynchronize();  // the parts are written
   if (w >= (int64_t)d.num_seqs * d.q_len * d.Hq) return;
   const int64_t grow = w / d.Hq;
   const int head = (int)(w % d.Hq), group = d.Hq / d.Hkv;
@@ -523,15 +516,31 @@ static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
   constexpr int merge = PA_WARPS * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
   constexpr int smem = ring > merge ? ring : merge;
   auto k = page_attn_kernel<KV, DH, NT>;
-  cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  PaPlan plan{tiles, 31, 0};
-  while ((1ll << (plan.shift - 31)) < d.page) ++plan.shift;
-  plan.magic = (uint32_t)(((1ull << plan.shift) + d.page - 1) / d.page);
-  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, plan);
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return check_launch("page_attention: shared memory");
+    ready.fetch_or(bit);
+  }
+  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, tiles, FastDiv(d.page));
   if (check_launch("page_attention")) return -1;
   if (d.nsplit == 1) return 0;
   const int64_t warps = (int64_t)d.num_seqs * d.q_len * d.Hq;
-  page_attn_join_kernel<DH><<<cdiv(warps * 32, 128), 128, 0, s>>>(d, 8 * NT, d.nsplit);
+  // launched while the parts still run (its blocks wait for them in the launch order of
+  // the stream): the launch's own latency is not waited for
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(cdiv(warps * 32, 128));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, page_attn_join_kernel<DH>, d, 8 * NT, d.nsplit);
   return check_launch("page_attention_join");
 }
 
@@ -541,15 +550,25 @@ using namespace lk;
 
 // Into how many parts a context may be cut, and the least units of a part, from the
 // longest context that the host expects (each block cuts its sequence's own length).
-// A block costs what 150 tokens cost beside its part (2.3 us), so parts are as few as
-// fill the GPU: 2.5 blocks an SM (1 reaches 60 % of the rate of 2 or 3), of 256 tokens
-// at least.  Where the sequences alone fill it, only contexts over 4096 are cut, so
-// that one of them does not run on alone.
+// The SM with the most blocks decides: k blocks each of a part, beside which a block
+// costs what 150 tokens cost (2.3 us); with k = 1 an SM reaches 60 % of the rate that it
+// has with 2 or 3 (two contexts of 100003 tokens: 105 us with 128 blocks, 72 with 288,
+// 74 with 432, 79 with 368, which leave some SMs 3 and some 2).  Where the sequences
+// alone fill the GPU only contexts over 4096 are cut, so that one does not run on alone
+// (256 sequences: 190 us uncut, 206 in halves, 227 in quarters).
 extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units) {
   const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
-  const int fill = (int)std::max<int64_t>(1, 5 * num_sms() / 2 / blocks), length = cdiv(max_ctx, 4096);
-  *nsplit = std::max(1, std::min(std::max(fill, length), cdiv(max_ctx, 256)));
-  *min_units = fill > 1 ? 256 / PA_UNIT : 4096 / PA_UNIT;
+  const int sms = num_sms(), most = std::max(1, cdiv(max_ctx, 256));
+  int best = 1;
+  double least = 1e30;
+  for (int k = 0; k <= (rows <= 8 ? 3 : 2); ++k) {
+    const int ns = (int)std::min<int64_t>(most, std::max<int64_t>(1, (int64_t)k * sms / blocks));
+    const int64_t load = (blocks * ns + sms - 1) / sms;
+    const double cost = load * ((double)max_ctx / ns + 150) * (load == 1 ? 1.6 : 1.0);
+    if (cost < least) least = cost, best = ns;
+  }
+  *nsplit = best > 1 ? best : std::max(1, cdiv(max_ctx, 4096));
+  *min_units = best > 1 ? 256 / PA_UNIT : 4096 / PA_UNIT;
 }
 
 extern "C" int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s) {

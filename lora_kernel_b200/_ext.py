@@ -65,22 +65,32 @@ def available() -> bool:
         return False
 
 
+_sm100 = set()  # devices seen to be sm_100
+
+
 def require_device(t: torch.Tensor) -> None:
+    if t.device in _sm100:
+        return
     if not t.is_cuda:
         raise RuntimeError("lora_kernel_b200 ops run on CUDA tensors only")
     major, _ = torch.cuda.get_device_capability(t.device)
     if major != 10:
         raise RuntimeError("lora_kernel_b200 kernels are built for sm_100a (B200) only")
+    _sm100.add(t.device)
 
 
 def status(device) -> torch.Tensor:
     """Per-device int32 status word shared by all kernels."""
+    t = _status.get(device)  # a torch.device with an index, as tensors have it
+    if t is not None:
+        return t
     device = torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    t = _status.get(idx)
+    key = torch.device("cuda", idx)
+    t = _status.get(key)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _status[idx] = t
+        t = torch.zeros(1, dtype=torch.int32, device=key)
+        _status[key] = t
     return t
 
 
