@@ -14,8 +14,8 @@ from .._ext import C, require_device, status
 
 
 def token_counts(rows: int, vocab: int, device="cuda") -> torch.Tensor:
-    """An empty table of token counts."""
-    return torch.zeros(rows, vocab, dtype=torch.int16, device=device)
+    """An empty table of token counts (rows padded to 16 bytes: a view of a wider table where vocab is odd)."""
+    return torch.zeros(rows, (vocab + 7) // 8 * 8, dtype=torch.int16, device=device)[:, :vocab]
 
 
 def set_token_counts(counts: torch.Tensor, rows: Optional[torch.Tensor], tokens: torch.Tensor, offsets: torch.Tensor,
