@@ -212,13 +212,24 @@ __global__ void __launch_bounds__(256) page_gather_kernel(LkPageGatherDesc d, in
 
 // ---------------------------------------------------------------- page copies
 // grid (moves * layers, tensors): a block copies one page of one layer of one
-// tensor.
+// tensor, four loads a thread on their way before the first store.  Bound by HBM.
+constexpr int COPY_THREADS = 128, COPY_AHEAD = 4;
+
 template <typename T>
 __device__ __forceinline__ void copy_as(const char* src, char* dst, int64_t bytes) {
-  for (int64_t i = threadIdx.x; i < bytes / (int64_t)sizeof(T); i += blockDim.x) ((T*)dst)[i] = ((const T*)src)[i];
+  const int64_t n = bytes / (int64_t)sizeof(T);
+  for (int64_t i = threadIdx.x; i < n; i += COPY_AHEAD * COPY_THREADS) {
+    T x[COPY_AHEAD];
+#pragma unroll
+    for (int k = 0; k < COPY_AHEAD; ++k)
+      if (i + k * COPY_THREADS < n) x[k] = ((const T*)src)[i + k * COPY_THREADS];
+#pragma unroll
+    for (int k = 0; k < COPY_AHEAD; ++k)
+      if (i + k * COPY_THREADS < n) ((T*)dst)[i + k * COPY_THREADS] = x[k];
+  }
 }
 
-__global__ void copy_pages_kernel(LkCopyPagesDesc d) {
+__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(LkCopyPagesDesc d) {
   const int m = blockIdx.x / d.layers, layer = blockIdx.x % d.layers;
   const int src = d.moves[2 * m], dst = d.moves[2 * m + 1];
   if (src < 0 || dst < 0 || src >= d.num_pages || dst >= d.num_pages) {
@@ -267,6 +278,6 @@ extern "C" int lk_page_gather(const LkPageGatherDesc* d, cudaStream_t s) {
 extern "C" int lk_copy_pages(const LkCopyPagesDesc* d, cudaStream_t s) {
   if (d->num_moves == 0 || d->layers == 0 || d->tensors == 0) return 0;
   LK_REQUIRE((int64_t)d->num_moves * d->layers < (1ll << 31), "copy_pages: too many moves in one call");
-  copy_pages_kernel<<<dim3(d->num_moves * d->layers, d->tensors), 256, 0, s>>>(*d);
+  copy_pages_kernel<<<dim3(d->num_moves * d->layers, d->tensors), COPY_THREADS, 0, s>>>(*d);
   return check_launch("copy_pages");
 }

@@ -14,17 +14,15 @@
 namespace lk {
 
 constexpr int ADJ_THREADS = 256;
-constexpr int ADJ_VECS = 2;                                // groups of 8 columns a thread
-constexpr int ADJ_CHUNK = ADJ_THREADS * ADJ_VECS * 8;  // columns a block
+constexpr int ADJ_STEP = ADJ_THREADS * 8;  // columns a block takes with one group of 8 a thread
+constexpr int ADJ_GROUPS = 2;              // groups a thread takes where there are many rows
 
-// z / r as z * (1 / r): a rounding of 2^-24 more
+// z / r as z * (1 / r): a rounding of 2^-24 more.  Without branches; a token not seen
+// (c = 0) keeps its bits (x * 1 - 0).
 __device__ __forceinline__ float adjusted(float x, uint32_t c, float r, float inv_r, float f, float p) {
-  if (c) {
-    const int made = c & 0x7FFF;
-    x *= x > 0.f ? inv_r : r;
-    if (made) x -= fmaf(f, (float)made, p);
-  }
-  return x;
+  const uint32_t made = c & 0x7FFFu;
+  const float scale = c ? (x > 0.f ? inv_r : r) : 1.f;
+  return fmaf(x, scale, made ? -fmaf(f, (float)made, p) : -0.f);
 }
 
 // 4 bits -> 4 bytes of 0xFF or 0
@@ -32,21 +30,29 @@ __device__ __forceinline__ uint32_t spread4(uint32_t bits) {
   return ((bits & 0xFu) * 0x00204081u & 0x01010101u) * 0xFFu;
 }
 
-// grid (chunks of the vocabulary, rows).  Bound by HBM: 6 bytes and a bit read or
-// written per bf16 logit, and 6 bytes a column leave no room for 40 instructions a
+// 8 columns of a row as loaded: pairs of bf16 or single floats, pairs of counts, mask bits
+template <bool F32>
+struct AdjGroup {
+  uint32_t x[F32 ? 8 : 4], c[4], allowed;
+};
+
+// grid (spans of the vocabulary, rows); a thread's G groups of 8 columns are all loaded
+// before anything else, which is what keeps enough bytes on their way.  Bound by HBM: 6 bytes and
+// a bit read or written per bf16 logit, which leaves no room for 40 instructions a
 // column: the logits stay packed, and only pairs of columns with a count or a bias are
 // taken apart (1 % of the columns are seen or biased in a request of some thousand
 // tokens: 40 % of a warp's pairs).  256 rows of 128256 with 300 biases each and masks
-// in %ADJ%.
+// in 43.5 us, 35 without biases (torch.add of the logits and the counts: 31); 1 or 4 groups,
+// 5 blocks an SM and blocks of 512 are 2-15 us slower.
 // VEC: every row of every table starts on 16 bytes; a thread takes 8 neighbouring
 // columns at a time.  Otherwise (an odd vocabulary without a padded pitch) its 8 lie a
 // block's width apart, one access each.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(ADJ_THREADS) adjust_logits_kernel(LkAdjustLogitsDesc d) {
+template <typename T, bool VEC, int G>
+__global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2) ? 6 : 3) adjust_logits_kernel(LkAdjustLogitsDesc d) {
   constexpr bool F32 = sizeof(T) == 4;
-  __shared__ float extra[ADJ_CHUNK];               // the row's biases in this chunk
-  __shared__ uint32_t biased[ADJ_CHUNK / 32];      // which columns have one
-  const int i = blockIdx.y, tid = threadIdx.x, v0 = blockIdx.x * ADJ_CHUNK, n = min(ADJ_CHUNK, d.vocab - v0);
+  extern __shared__ __align__(16) float extra[];  // the row's biases in this span, then a bit per column that has one
+  uint32_t* biased = reinterpret_cast<uint32_t*>(extra + G * ADJ_STEP);
+  const int i = blockIdx.y, tid = threadIdx.x, v0 = blockIdx.x * G * ADJ_STEP, n = min(G * ADJ_STEP, d.vocab - v0);
   const T* in = (const T*)d.logits + (int64_t)i * d.ld + v0;
   T* out = (T*)d.out + (int64_t)i * d.ldo + v0;
   int row = d.counts ? (d.rows ? d.rows[i] : i) : -1;
@@ -59,60 +65,61 @@ __global__ void __launch_bounds__(ADJ_THREADS) adjust_logits_kernel(LkAdjustLogi
   }
   const int16_t* counts = d.counts + (row >= 0 ? row * d.ldc + v0 : 0);
   const int* mask = d.mask + (mrow >= 0 ? mrow * d.ldm + v0 / 32 : 0);  // v0 is a multiple of 32
-  // column k of this thread's group g
-  auto col = [&](int g, int k) { return VEC ? (g * ADJ_THREADS + tid) * 8 + k : (g * 8 + k) * ADJ_THREADS + tid; };
-
-  // everything is loaded first: x holds pairs of bf16 or single floats, c pairs of counts
-  uint32_t x[ADJ_VECS][F32 ? 8 : 4], c[ADJ_VECS][4], allowed[ADJ_VECS];
-#pragma unroll
-  for (int g = 0; g < ADJ_VECS; ++g) {
-    if (VEC && col(g, 0) + 8 <= n) {
+  // column k of this thread in the group that begins at column s
+  auto col = [&](int s, int k) { return s + (VEC ? tid * 8 + k : k * ADJ_THREADS + tid); };
+  auto load = [&](int s) {
+    AdjGroup<F32> g;
+    if (VEC && col(s, 0) + 8 <= n) {
 #pragma unroll
       for (int q = 0; q < (F32 ? 2 : 1); ++q) {
-        const uint4 a = reinterpret_cast<const uint4*>(in + col(g, 0))[q];
-        x[g][4 * q] = a.x, x[g][4 * q + 1] = a.y, x[g][4 * q + 2] = a.z, x[g][4 * q + 3] = a.w;
+        const uint4 a = reinterpret_cast<const uint4*>(in + col(s, 0))[q];
+        g.x[4 * q] = a.x, g.x[4 * q + 1] = a.y, g.x[4 * q + 2] = a.z, g.x[4 * q + 3] = a.w;
       }
       uint4 a = make_uint4(0, 0, 0, 0);
-      if (row >= 0) a = *reinterpret_cast<const uint4*>(counts + col(g, 0));
-      c[g][0] = a.x, c[g][1] = a.y, c[g][2] = a.z, c[g][3] = a.w;
-      allowed[g] = mrow >= 0 ? reinterpret_cast<const uint8_t*>(mask)[col(g, 0) / 8] : 0xFFu;
+      if (row >= 0) a = *reinterpret_cast<const uint4*>(counts + col(s, 0));
+      g.c[0] = a.x, g.c[1] = a.y, g.c[2] = a.z, g.c[3] = a.w;
+      g.allowed = mrow >= 0 ? reinterpret_cast<const uint8_t*>(mask)[col(s, 0) / 8] : 0xFFu;
     } else {
-      allowed[g] = 0;
+      g.allowed = 0;
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
         uint32_t xw[2] = {0, 0}, cw[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int j = col(g, k + q);
+          const int j = col(s, k + q);
           if (j < n) {
             if constexpr (F32) xw[q] = __float_as_uint(in[j]);
             else xw[q] = __bfloat16_as_ushort(in[j]);
             if (row >= 0) cw[q] = (uint16_t)counts[j];
-            if (mrow < 0 || (mask[j / 32] >> (j & 31) & 1)) allowed[g] |= 1u << (k + q);
+            if (mrow < 0 || (mask[j / 32] >> (j & 31) & 1)) g.allowed |= 1u << (k + q);
           }
         }
-        if constexpr (F32) x[g][k] = xw[0], x[g][k + 1] = xw[1];
-        else x[g][k / 2] = xw[0] | xw[1] << 16;
-        c[g][k / 2] = cw[0] | cw[1] << 16;
+        if constexpr (F32) g.x[k] = xw[0], g.x[k + 1] = xw[1];
+        else g.x[k / 2] = xw[0] | xw[1] << 16;
+        g.c[k / 2] = cw[0] | cw[1] << 16;
       }
     }
-  }
+    return g;
+  };
+  AdjGroup<F32> groups[G];
+#pragma unroll
+  for (int s = 0; s < G; ++s) groups[s] = load(s * ADJ_STEP);
   const float r = row >= 0 ? d.penalties[3 * i] : 1.f, f = row >= 0 ? d.penalties[3 * i + 1] : 0.f,
               p = row >= 0 ? d.penalties[3 * i + 2] : 0.f;
 
-  int any = 0;  // a bias falls into this chunk
+  int any = 0;  // a bias falls into this span
   if (b0 < b1) {
-    for (int j = tid; j < ADJ_CHUNK / 4; j += ADJ_THREADS) reinterpret_cast<float4*>(extra)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (tid < ADJ_CHUNK / 32) biased[tid] = 0;
+    constexpr int words = G * (ADJ_STEP + ADJ_STEP / 32) / 4;
+    for (int j = tid; j < words; j += ADJ_THREADS) reinterpret_cast<float4*>(extra)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();
     for (int j = b0 + tid; j < b1; j += ADJ_THREADS) {
       const int id = d.bias_ids[j], at = id - v0;
-      if ((unsigned)id >= (unsigned)d.vocab) {
-        if (blockIdx.x == 0 && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-      } else if (at >= 0 && at < n) {
+      if ((unsigned)at < (unsigned)n) {
         atomicAdd(&extra[at], d.bias_values[j]);
         atomicOr(&biased[at / 32], 1u << (at & 31));
         any = 1;
+      } else if (blockIdx.x == 0 && (unsigned)id >= (unsigned)d.vocab && d.status) {
+        atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
       }
     }
     any = __syncthreads_or(any);
@@ -120,65 +127,67 @@ __global__ void __launch_bounds__(ADJ_THREADS) adjust_logits_kernel(LkAdjustLogi
 
   const float inv_r = 1.f / r;
 #pragma unroll
-  for (int g = 0; g < ADJ_VECS; ++g) {
+  for (int e = 0; e < G; ++e) {
+    const int s = e * ADJ_STEP;
+    AdjGroup<F32>& g = groups[e];
     uint32_t bias_bits = 0;
     if (any) {
       if constexpr (VEC) {
-        bias_bits = reinterpret_cast<const uint8_t*>(biased)[col(g, 0) / 8];
+        bias_bits = reinterpret_cast<const uint8_t*>(biased)[col(s, 0) / 8];
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) bias_bits |= (biased[col(g, k) / 32] >> (col(g, k) & 31) & 1) << k;
+        for (int k = 0; k < 8; ++k) bias_bits |= (biased[col(s, k) / 32] >> (col(s, k) & 31) & 1) << k;
       }
     }
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
-      if (c[g][k / 2] | (bias_bits >> k & 3)) {
+      if (g.c[k / 2] | (bias_bits >> k & 3)) {
         float y[2];
-        if constexpr (F32) y[0] = __uint_as_float(x[g][k]), y[1] = __uint_as_float(x[g][k + 1]);
-        else y[0] = __uint_as_float(x[g][k / 2] << 16), y[1] = __uint_as_float(x[g][k / 2] & 0xFFFF0000u);
+        if constexpr (F32) y[0] = __uint_as_float(g.x[k]), y[1] = __uint_as_float(g.x[k + 1]);
+        else y[0] = __uint_as_float(g.x[k / 2] << 16), y[1] = __uint_as_float(g.x[k / 2] & 0xFFFF0000u);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          y[q] = adjusted(y[q], c[g][k / 2] >> (16 * q) & 0xFFFFu, r, inv_r, f, p);
-          if (bias_bits >> (k + q) & 1) y[q] += extra[col(g, k + q)];
+          y[q] = adjusted(y[q], g.c[k / 2] >> (16 * q) & 0xFFFFu, r, inv_r, f, p);
+          if (bias_bits >> (k + q) & 1) y[q] += extra[col(s, k + q)];
         }
-        if constexpr (F32) x[g][k] = __float_as_uint(y[0]), x[g][k + 1] = __float_as_uint(y[1]);
-        else x[g][k / 2] = pack_bf16x2(y[0], y[1]);
+        if constexpr (F32) g.x[k] = __float_as_uint(y[0]), g.x[k + 1] = __float_as_uint(y[1]);
+        else g.x[k / 2] = pack_bf16x2(y[0], y[1]);
       }
     }
     if (mrow >= 0) {
       if constexpr (F32) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (!(allowed[g] >> k & 1)) x[g][k] = 0xFF800000u;
+          if (!(g.allowed >> k & 1)) g.x[k] = 0xFF800000u;
       } else {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const uint32_t keep = spread4(allowed[g] >> (4 * q));
+          const uint32_t keep = spread4(g.allowed >> (4 * q));
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const uint32_t m = __byte_perm(keep, 0, k ? 0x3322 : 0x1100);
-            x[g][2 * q + k] = (x[g][2 * q + k] & m) | (~m & 0xFF80FF80u);
+            g.x[2 * q + k] = (g.x[2 * q + k] & m) | (~m & 0xFF80FF80u);
           }
         }
       }
     }
-    if (VEC && col(g, 0) + 8 <= n) {
+    if (VEC && col(s, 0) + 8 <= n) {
 #pragma unroll
       for (int q = 0; q < (F32 ? 2 : 1); ++q)
-        reinterpret_cast<uint4*>(out + col(g, 0))[q] = make_uint4(x[g][4 * q], x[g][4 * q + 1], x[g][4 * q + 2], x[g][4 * q + 3]);
+        reinterpret_cast<uint4*>(out + col(s, 0))[q] = make_uint4(g.x[4 * q], g.x[4 * q + 1], g.x[4 * q + 2], g.x[4 * q + 3]);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (col(g, k) < n) {
-          if constexpr (F32) out[col(g, k)] = __uint_as_float(x[g][k]);
-          else out[col(g, k)] = __ushort_as_bfloat16((unsigned short)(x[g][k / 2] >> (16 * (k & 1))));
+        if (col(s, k) < n) {
+          if constexpr (F32) out[col(s, k)] = __uint_as_float(g.x[k]);
+          else out[col(s, k)] = __ushort_as_bfloat16((unsigned short)(g.x[k / 2] >> (16 * (k & 1))));
         }
     }
   }
 }
 
 constexpr int CNT_THREADS = 512;
-constexpr int CNT_CHUNK = 8192;  // vocabulary columns per block (a 32 KB histogram)
+constexpr int CNT_CHUNK = 4096;  // vocabulary columns per block (a 16 KB histogram)
 
 // grid (chunks, sequences): histogram of a sequence's history over the block's
 // vocabulary columns in shared memory, written over the row.  Every chunk reads the
@@ -211,15 +220,16 @@ __global__ void __launch_bounds__(CNT_THREADS) set_token_counts_kernel(LkTokenCo
     const uint32_t c = hist[j];
     return min(c & 0x7FFFFFFFu, 32767u) | (c >> 31 << 15);
   };
-  for (int j = threadIdx.x * 8; j < n; j += CNT_THREADS * 8) {
-    if (vec && j + 8 <= n) {
+  if (vec) {
+    for (int j = threadIdx.x * 8; j < n; j += CNT_THREADS * 8) {
       uint32_t w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = packed(j + 2 * k) | packed(j + 2 * k + 1) << 16;
-      *reinterpret_cast<uint4*>(out + j) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      for (int k = j; k < min(j + 8, n); ++k) out[k] = (int16_t)packed(k);
+      if (j + 8 <= n) *reinterpret_cast<uint4*>(out + j) = make_uint4(w[0], w[1], w[2], w[3]);
+      else for (int k = j; k < n; ++k) out[k] = (int16_t)packed(k);
     }
+  } else {
+    for (int j = threadIdx.x; j < n; j += CNT_THREADS) out[j] = (int16_t)packed(j);
   }
 }
 
@@ -256,16 +266,20 @@ using namespace lk;
 extern "C" int lk_adjust_logits(const LkAdjustLogitsDesc* d, cudaStream_t s) {
   if (d->n == 0 || d->vocab == 0) return 0;
   LK_REQUIRE(d->n <= 65535, "adjust_logits: at most 65535 rows");
-  const dim3 grid(cdiv(d->vocab, ADJ_CHUNK), d->n);
   const int each = d->f32 ? 4 : 2;
   const bool vec = rows_aligned(d->logits, d->ld, each, d->n) && rows_aligned(d->out, d->ldo, each, d->n) &&
                    (!d->counts || rows_aligned(d->counts, d->ldc, 2, d->count_rows));
-  if (d->f32)
-    vec ? adjust_logits_kernel<float, true><<<grid, ADJ_THREADS, 0, s>>>(*d)
-        : adjust_logits_kernel<float, false><<<grid, ADJ_THREADS, 0, s>>>(*d);
-  else
-    vec ? adjust_logits_kernel<__nv_bfloat16, true><<<grid, ADJ_THREADS, 0, s>>>(*d)
-        : adjust_logits_kernel<__nv_bfloat16, false><<<grid, ADJ_THREADS, 0, s>>>(*d);
+  // long spans share the search for a row's biases and have more loads on their way; short
+  // ones fill the GPU
+  const int groups = (int64_t)d->n * cdiv(d->vocab, ADJ_GROUPS * ADJ_STEP) >= 4 * num_sms() ? ADJ_GROUPS : 1;
+  const dim3 grid(cdiv(d->vocab, groups * ADJ_STEP), d->n);
+  const int smem = d->bias_offsets ? groups * (ADJ_STEP + ADJ_STEP / 32) * 4 : 0;
+#define LK_ADJ(T, VEC)                                                                           \
+  (groups == 1 ? adjust_logits_kernel<T, VEC, 1><<<grid, ADJ_THREADS, smem, s>>>(*d)             \
+               : adjust_logits_kernel<T, VEC, ADJ_GROUPS><<<grid, ADJ_THREADS, smem, s>>>(*d))
+  if (d->f32) vec ? LK_ADJ(float, true) : LK_ADJ(float, false);
+  else vec ? LK_ADJ(__nv_bfloat16, true) : LK_ADJ(__nv_bfloat16, false);
+#undef LK_ADJ
   return check_launch("adjust_logits");
 }
 
