@@ -7,7 +7,7 @@
   bench  [--gpus N --steps K --warmup W]   the headline training benchmark
          [--kernels]                       kernel micro-benchmarks instead
          [--serve ...]                     serving load generator
-  serve  --preset NAME [--port P] [--weights int4|int8|fp8|none] [--kv fp8|int8|bf16]
+  serve  --preset NAME [--port P] [--weights int4|int8|fp8|none] [--kv fp8|int8|bf16|fp8_page|int8_page]
          [--replicas N --replica-policy prefix_affinity|least_loaded|round_robin]
   export --out PATH [--format gguf|hf|onnx] [--dtype bf16|f16|f32] [--checkpoint model.safetensors]
   env    versions, GPU, NVLink, extension status

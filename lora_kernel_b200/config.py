@@ -154,7 +154,7 @@ class ParallelConfig:
 class QuantConfig:
     weights: str = "none"  # none|int8|int4|fp8
     group_size: int = 128
-    kv_cache: str = "bf16"  # bf16|fp8|int8
+    kv_cache: str = "bf16"  # bf16|fp8|int8 (a scale per token and head)|fp8_page|int8_page (per page and head)
 
 
 @dataclass

@@ -10,7 +10,13 @@ Scheduler (one `step()` = one decode batch plus prefill chunks):
     step's token budget (max_num_batched_tokens) and free KV blocks allow;
     long prompts are split into chunks (chunked prefill) so one huge prompt
     does not stall the decode batch;
-  * prompt blocks already in the prefix cache are not recomputed.
+  * prompt blocks already in the prefix cache are not recomputed;
+  * a request for n samples becomes n requests when its prompt is computed: the
+    others fork its block table (full blocks shared, the partial one copied on the
+    device) and sample their first token from the same logits;
+  * penalties, biases and grammar masks change the logits of the requests that
+    have any before sampling; each such request holds a row of the runner's
+    table of token counts while it runs.
 
 Reference: ContinuousBatching (include/nn/inference.hpp:89-170, FIFO admit to
 max_batch), DynamicBatcher / PriorityScheduler
@@ -22,8 +28,8 @@ from __future__ import annotations
 import itertools
 import time
 from collections import deque
-from dataclasses import dataclass, field
-from typing import Callable, Dict, List, Optional
+from dataclasses import dataclass, field, replace
+from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
 
@@ -44,6 +50,34 @@ class SamplingParams:
     # server's OpenAI `stop` strings, tokenized); the server leaves them out of the text
     stop_sequences: tuple = ()
     seed: Optional[int] = None
+    # logits before sampling (ops/logits.py): z / r or z * r for tokens of the prompt or
+    # output, - frequency * count - presence for generated ones, + bias per token id,
+    # and -inf for all but the allowed tokens: a fixed set, or a grammar called with
+    # the tokens generated so far (it returns the ids allowed next, None = all; none at
+    # all ends the request with reason "stop" and without a token)
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: Optional[Dict[int, float]] = None
+    allowed_token_ids: Optional[Sequence[int]] = None
+    grammar: Optional[Callable[[List[int]], Optional[Sequence[int]]]] = None
+    n: int = 1  # samples of the prompt; the request's own is the first (Request.samples: the others' ids)
+
+    @property
+    def penalised(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0
+
+    @property
+    def adjusts(self) -> bool:
+        return self.penalised or bool(self.logit_bias) or self.allowed_token_ids is not None or self.grammar is not None
+
+    def allowed(self, output: List[int]) -> Optional[Sequence[int]]:
+        """The token ids that may come next (None = all)."""
+        ids = self.grammar(output) if self.grammar is not None else None
+        if ids is None or self.allowed_token_ids is None:
+            return self.allowed_token_ids if ids is None else ids
+        fixed = set(self.allowed_token_ids)
+        return [t for t in ids if t in fixed]
 
 
 def _mix64(a: int, b: int) -> int:
@@ -80,6 +114,8 @@ class Request:
     finished: bool = False
     finish_reason: Optional[str] = None
     on_token: Optional[Callable[["Request", int], None]] = None
+    samples: List[int] = field(default_factory=list)  # ids of the other samples (params.n > 1)
+    counts_row: int = -1        # row of the runner's token counts
 
     @property
     def tokens(self) -> List[int]:
@@ -123,6 +159,8 @@ class LLMEngine:
         self.stats = {"prompt_tokens": 0, "generated_tokens": 0, "preemptions": 0, "steps": 0,
                       "prefill_tokens_computed": 0}
         self._seed = 1234
+        self._counts_free: List[int] = []  # unused rows of the runner's token counts
+        self._counts_rows = 0
         # when a list: one (schedule_s, prefill_s, decode_s, prefill_tokens,
         # decode_seqs) record per step, host clock; the prefill and decode
         # phases each end with the device read of their sampled tokens
@@ -141,6 +179,8 @@ class LLMEngine:
                                  "from vocabulary slices); use top_p = 1")
             if params.seed is not None:
                 raise ValueError("per-request seeds are not supported by this runner (tensor-parallel serving)")
+        if params is not None:
+            self._check_params(params)
         r = Request(next(self.ids), list(prompt), params or SamplingParams(), priority,
                     self.clock() if arrival is None else arrival, on_token=on_token)
         self.stats["prompt_tokens"] += len(prompt)
@@ -151,13 +191,28 @@ class LLMEngine:
         self.waiting.insert(idx, r)
         return r.req_id
 
+    def _check_params(self, p: SamplingParams) -> None:
+        if p.adjusts and not getattr(self.runner, "supports_adjust", False):
+            raise ValueError("penalties, biases and grammars are not supported by this runner (tensor-parallel serving "
+                             "samples from vocabulary slices)")
+        if not (p.repetition_penalty > 0 and abs(p.frequency_penalty) < float("inf") and abs(p.presence_penalty) < float("inf")
+                and p.repetition_penalty < float("inf")):
+            raise ValueError("penalties must be finite, repetition_penalty above 0")
+        V = self.cfg.vocab_size
+        if any(not 0 <= t < V for t in p.logit_bias or ()) or any(not 0 <= t < V for t in p.allowed_token_ids or ()):
+            raise ValueError(f"logit_bias and allowed_token_ids take token ids in [0, {V})")
+        if p.allowed_token_ids is not None and not len(p.allowed_token_ids):
+            raise ValueError("allowed_token_ids must not be empty")
+        if not 1 <= p.n <= self.sc.max_num_seqs:
+            raise ValueError(f"n must be in [1, {self.sc.max_num_seqs}]")
+
     def abort_request(self, req_id: int) -> bool:
         """Drop a request that has not finished (its client went away): its KV
         blocks are freed and it leaves the waiting / running queues.  Returns
         False when the request is unknown or already finished."""
         for r in list(self.running):
             if r.req_id == req_id:
-                self.blocks.free_seq(r.table)
+                self._release(r)
                 self.running.remove(r)
                 r.finished, r.finish_reason = True, "abort"
                 self.finished[r.req_id] = r
@@ -172,6 +227,63 @@ class LLMEngine:
                 return True
         return False
 
+    # ------------------------------------------------------------ forks, pages
+    def fork_request(self, req_id: int, params: Optional[SamplingParams] = None, on_token=None) -> int:
+        """Continue a running request a second time from where it is now: a new
+        request with the same tokens so far, whose KV blocks are shared with the
+        first's (the partly filled one copied).  params: the new one's (default:
+        the same with another seed)."""
+        r = next((x for x in self.running if x.req_id == req_id), None)
+        if r is None or r.in_prefill or not r.output:
+            raise ValueError("fork_request: the request is not running, or has no token yet")
+        if params is not None:
+            if params.n != 1:
+                raise ValueError("fork_request: n must be 1")
+            if len(r.prompt) + params.max_tokens > self.sc.max_model_len:
+                raise ValueError("prompt + max_tokens exceeds max_model_len")
+            self._check_params(params)
+        return self._fork(r, r.n_tokens - 1, params, on_token).req_id
+
+    def _fork(self, r: Request, computed: int, params: Optional[SamplingParams], on_token) -> Request:
+        """A copy of r whose first `computed` tokens are in the cache; it runs at once
+        where there is room, else it waits and is recomputed (from the prefix cache)."""
+        rid = next(self.ids)
+        if params is None:
+            seed = None if r.params.seed is None else _mix64(r.params.seed, rid) >> 1
+            params = replace(r.params, n=1, seed=seed)
+        c = Request(rid, list(r.prompt), params, r.priority, self.clock(), output=list(r.output),
+                    cached_prefix=computed, on_token=on_token, first_token_time=r.first_token_time,
+                    token_times=list(r.token_times))
+        if hasattr(self.runner, "copy_pages") and len(self.running) < self.sc.max_num_seqs:
+            try:
+                c.table, copies = self.blocks.fork(r.table, computed)
+            except MemoryError:
+                pass
+            else:
+                self.runner.copy_pages(copies)
+                c.prefill_len = c.computed = computed
+                c.scheduled_time = c.arrival
+                self.running.append(c)
+                return c
+        self.waiting.appendleft(c)
+        return c
+
+    def compact(self) -> int:
+        """Move the KV blocks in use to the lowest block ids (between steps);
+        returns how many moved."""
+        if not hasattr(self.runner, "copy_pages"):
+            raise ValueError("compact is not supported by this runner")
+        moves = self.blocks.compact([r.table for r in self.running] + [r.table for r in self.waiting])
+        self.runner.copy_pages(moves)
+        return len(moves)
+
+    def _release(self, r: Request) -> None:
+        """What a request holds while it runs: its KV blocks and its counts row."""
+        self.blocks.free_seq(r.table)
+        if r.counts_row >= 0:
+            self._counts_free.append(r.counts_row)
+            r.counts_row = -1
+
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
 
@@ -179,7 +291,7 @@ class LLMEngine:
     def _preempt(self, r: Request) -> None:
         """Free a running request's blocks; it is recomputed when readmitted
         (prompt and generated tokens, except the last one, which decode feeds)."""
-        self.blocks.free_seq(r.table)
+        self._release(r)
         r.computed = 0
         self.running.remove(r)
         self.waiting.appendleft(r)
@@ -237,7 +349,13 @@ class LLMEngine:
         return decode, items
 
     # ---------------------------------------------------------------- step
-    def _emit(self, r: Request, tok: int, now: float) -> None:
+    def _emit(self, r: Request, tok: Optional[int], now: float) -> None:
+        if tok is None:  # its grammar allows no token
+            r.finished, r.finish_reason = True, "stop"
+            self._release(r)
+            self.running.remove(r)
+            self.finished[r.req_id] = r
+            return
         r.output.append(tok)
         r.token_times.append(now)
         if r.first_token_time is None:
@@ -250,14 +368,40 @@ class LLMEngine:
         if r.on_token:
             r.on_token(r, tok)
         if r.finished:
-            self.blocks.free_seq(r.table)
+            self._release(r)
             self.running.remove(r)
             self.finished[r.req_id] = r
 
-    def _sample(self, reqs: List[Request], logits: torch.Tensor) -> List[int]:
+    def _adjust(self, reqs: List[Request], logits: torch.Tensor, allowed: List) -> torch.Tensor:
+        """Penalties, biases and masks of the requests that have any; a request new to
+        the counts table (or back in it) gets its row written from its tokens."""
+        if not any(r.params.adjusts for r in reqs):
+            return logits
+        fresh = [r for r in reqs if r.params.penalised and r.counts_row < 0]
+        for r in fresh:
+            if not self._counts_free:  # one row per running request is enough
+                self._counts_free += range(self._counts_rows, self._counts_rows + self.sc.max_num_seqs)
+                self._counts_rows += self.sc.max_num_seqs
+            r.counts_row = self._counts_free.pop()
+        if fresh:
+            self.runner.set_counts([r.counts_row for r in fresh], [(r.prompt, r.output) for r in fresh], self._counts_rows)
+        ps = [r.params for r in reqs]
+        return self.runner.adjust_logits(
+            logits, [r.counts_row if r.params.penalised else -1 for r in reqs],
+            [(p.repetition_penalty, p.frequency_penalty, p.presence_penalty) for p in ps],
+            [p.logit_bias for p in ps], allowed)
+
+    def _sample(self, reqs: List[Request], logits: torch.Tensor) -> List[Optional[int]]:
+        allowed = [r.params.allowed(r.output) if r.params.adjusts else None for r in reqs]
+        tok = self._draw(reqs, self._adjust(reqs, logits, allowed))
+        if any(r.counts_row >= 0 for r in reqs):
+            self.runner.add_counts([r.counts_row for r in reqs], tok)
+        return [t if a is None or len(a) else None for t, a in zip(tok.tolist(), allowed)]
+
+    def _draw(self, reqs: List[Request], logits: torch.Tensor) -> torch.Tensor:
         temps = [r.params.temperature for r in reqs]
         if all(t <= 0 for t in temps):
-            tok = self.runner.sample(logits, None, 0)
+            return self.runner.sample(logits, None, 0)
         else:
             self._seed += 1
             kw = {}
@@ -268,8 +412,7 @@ class LLMEngine:
                 # a seeded request's draw k uses (its seed, k), whatever its batch row
                 kw["row_seeds"] = [_mix64(r.params.seed, len(r.output)) if r.params.seed is not None
                                    else _mix64(self._seed, i) for i, r in enumerate(reqs)]
-            tok = self.runner.sample(logits, temps, self._seed, **kw)
-        return tok.tolist()
+            return self.runner.sample(logits, temps, self._seed, **kw)
 
     def step(self) -> List[Request]:
         """Run one scheduling step; returns requests that finished during it."""
@@ -289,6 +432,8 @@ class LLMEngine:
             if seq_ids:
                 by_id = {r.req_id: r for r, _ in items}
                 reqs = [by_id[i] for i in seq_ids]
+                if any(r.params.n > 1 for r in reqs):
+                    reqs, logits = self._spread(reqs, logits)
                 toks = self._sample(reqs, logits)
                 now = self.clock()
                 for r, t in zip(reqs, toks):
@@ -312,8 +457,28 @@ class LLMEngine:
             self.step_log.append((t1 - t0, t2 - t1, t3 - t2, n_pre, len(decode)))
         return [self.finished[i] for i in self.finished if i not in done_before]
 
-    def generate(self, prompts: List[List[int]], params: Optional[SamplingParams] = None) -> List[List[int]]:
+    def _spread(self, reqs: List[Request], logits: torch.Tensor):
+        """Prompts just computed whose requests want several samples: the others are
+        forked and take the same row of logits (those that have to wait for room
+        are left to their own turn)."""
+        out, rows = [], []
+        for k, r in enumerate(reqs):
+            out.append(r)
+            rows.append(k)
+            if r.params.n > 1 and not r.samples:
+                for _ in range(r.params.n - 1):
+                    c = self._fork(r, r.prefill_len, None, r.on_token)
+                    r.samples.append(c.req_id)
+                    if c.table:
+                        out.append(c)
+                        rows.append(k)
+        return out, logits.index_select(0, torch.tensor(rows, device=logits.device))
+
+    def generate(self, prompts: List[List[int]], params: Optional[SamplingParams] = None) -> List:
+        """The outputs of the prompts; with params.n > 1, the list of its samples for each prompt."""
         ids = [self.add_request(p, params) for p in prompts]
-        while any(i not in self.finished for i in ids):
+        while any(i not in self.finished or any(j not in self.finished for j in self.finished[i].samples) for i in ids):
             self.step()
+        if params is not None and params.n > 1:
+            return [[self.finished[j].output for j in [i] + self.finished[i].samples] for i in ids]
         return [self.finished[i].output for i in ids]

@@ -6,7 +6,8 @@ block is identified by a hash chain over the token ids of all blocks up to and
 including it, so two prompts with the same first k blocks share k physical
 blocks (reference counted); a shared block is never written again (only full
 blocks are shared, a sequence's partial tail block is always private), so no
-copy-on-write is needed.  Unreferenced cached blocks stay reusable until the
+copy-on-write is needed.  A fork shares the full blocks too and gets a copy of
+the partial one.  Unreferenced cached blocks stay reusable until the
 allocator needs them back (least recently used first).
 
 Reference: PagedKVCache (include/nn/kv_cache.hpp:103-219: one global page
@@ -133,6 +134,45 @@ class BlockManager:
         if bi == len(table):
             table.append(self._take())
         return table[bi] * self.block_size + off
+
+    def fork(self, table: List[int], num_tokens: int) -> Tuple[List[int], List[Tuple[int, int]]]:
+        """Block table of a second sequence that starts with the first num_tokens
+        tokens of `table`, and the (source, destination) blocks to copy: full
+        blocks are shared, a partly filled one is copied."""
+        full, rest = divmod(num_tokens, self.block_size)
+        copies: List[Tuple[int, int]] = []
+        if rest:
+            copies.append((table[full], self._take()))  # before the sharing: it may find no block
+        child = table[:full]
+        for b in child:
+            self.ref[b] += 1
+        return child + [d for _, d in copies], copies
+
+    def compact(self, tables: Sequence[List[int]]) -> List[Tuple[int, int]]:
+        """Renumber the blocks in use (by sequences or the prefix cache) to the
+        lowest ids: updates `tables`, which must be the tables of all sequences,
+        and returns the (source, destination) blocks to copy.  No destination is
+        in use, so the copies can run in any order."""
+        held = [0] * self.num_blocks
+        for t in tables:
+            for b in t:
+                held[b] += 1
+        if held != self.ref:
+            raise ValueError("compact: the tables are not those of all sequences")
+        used = [b for b in range(self.num_blocks) if self.ref[b] or b in self.hash_of]
+        n = len(used)
+        holes = sorted(set(range(n)).difference(used))
+        moves = list(zip([b for b in used if b >= n], holes))
+        to = dict(moves)
+        for t in tables:
+            t[:] = [to.get(b, b) for b in t]
+        for s, d in moves:
+            self.ref[d], self.ref[s] = self.ref[s], 0
+        self.hash_of = {to.get(b, b): h for b, h in self.hash_of.items()}
+        self.block_of = {h: to.get(b, b) for h, b in self.block_of.items()}
+        self.evictable = OrderedDict((to.get(b, b), None) for b in self.evictable)
+        self.free = deque(range(n, self.num_blocks))
+        return moves
 
     def free_seq(self, table: List[int]) -> None:
         for b in table:

@@ -12,7 +12,15 @@ cache of every layer and runs two kinds of batches:
             K15 append, then K13 paged decode attention straight over the
             (fp8 / int8 / bf16) pages.
 
-The LM head runs only on each sequence's last row; K19 samples the next token.
+With kv_dtype "fp8_page" / "int8_page" the cache has one power-of-two scale per
+(page, KV head) instead of one per (token, KV head) (ops/paged.py): appends,
+decode attention (tensor cores) and the read-back for prefill go through its
+kernels, and chunks of up to PAGE_ATTN_ROWS tokens (speculative verification, the
+end of a prompt whose beginning is cached) attend to the pages directly.
+
+The LM head runs only on each sequence's last row; K19 samples the next token,
+after the penalties, biases and grammar masks of the requests that have any
+(ops/logits.py).
 Weights can stay bf16 (tcgen05 GEMM, SwiGLU fused into the gate|up epilogue)
 or be int8 / fp8 per row or int4 group-128 (K14: dequantising GEMV for
 decode-sized batches, dequantise + tcgen05 GEMM for prefill-sized ones).
@@ -31,7 +39,9 @@ from ..config import TransformerConfig
 from ..models.params import FlatParams
 from ..ops import elementwise as E
 from ..ops import gemm as G
+from ..ops import logits as LG
 from ..ops import norm as N
+from ..ops import paged as PG
 from ..ops import serving as SV
 from ..ops.attention import attention_fwd
 
@@ -61,23 +71,28 @@ class ModelRunner:
         self._scratch: Optional[torch.Tensor] = None
         self._load_weights(params, weights, group_size)
         H, KV, Dh = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
-        per_token = 2 * cfg.num_layers * KV * Dh * (2 if kv_dtype == "bf16" else 1)
-        per_token += 2 * cfg.num_layers * KV * 4 if kv_dtype != "bf16" else 0
+        self.page_scaled = kv_dtype in PG.PAGE_KV
+        per_block = 2 * cfg.num_layers * KV * Dh * (2 if kv_dtype == "bf16" else 1) * block_size
+        if kv_dtype != "bf16":
+            per_block += 2 * cfg.num_layers * KV * 4 * (1 if self.page_scaled else block_size)
         if num_blocks <= 0:
             free, _ = torch.cuda.mem_get_info(self.device)
-            num_blocks = max(16, int(free * mem_fraction) // (per_token * block_size))
+            num_blocks = max(16, int(free * mem_fraction) // per_block)
         self.num_blocks = num_blocks
         # one extra block at the end: the KV sink of padding rows in graph-captured decode
         slots = (num_blocks + 1) * block_size
         self.dummy_block = num_blocks
-        dt = SV.KV_TORCH[kv_dtype]
-        self.k_cache = torch.zeros(cfg.num_layers, slots, KV, Dh, dtype=dt, device=self.device)
-        self.v_cache = torch.zeros_like(self.k_cache)
-        if kv_dtype != "bf16":
-            self.k_scale = torch.zeros(cfg.num_layers, slots, KV, dtype=torch.float32, device=self.device)
-            self.v_scale = torch.zeros_like(self.k_scale)
+        if self.page_scaled:
+            self.k_cache, self.v_cache, self.k_scale, self.v_scale = PG.new_page_cache(
+                cfg.num_layers, num_blocks + 1, block_size, KV, Dh, kv_dtype, self.device)
         else:
+            dt = SV.KV_TORCH[kv_dtype]
+            self.k_cache = torch.zeros(cfg.num_layers, slots, KV, Dh, dtype=dt, device=self.device)
+            self.v_cache = torch.zeros_like(self.k_cache)
             self.k_scale = self.v_scale = None
+            if kv_dtype != "bf16":
+                self.k_scale = torch.zeros(cfg.num_layers, slots, KV, dtype=torch.float32, device=self.device)
+                self.v_scale = torch.zeros_like(self.k_scale)
         self.rope = E.rope_table(max_model_len, Dh, cfg.rope_base, self.device)
         self.use_graphs = False
         self._graphs: Dict[int, Tuple] = {}
@@ -139,14 +154,29 @@ class ModelRunner:
         xn, _, _ = N.rmsnorm_fwd(h, self.W[p + "attn_norm"], cfg.norm_eps)
         qkv = self._linear(xn, p + "wqkv")
         E.rope_(qkv, 0, cfg.num_heads + cfg.num_kv_heads, cfg.head_dim, self.rope, positions=pos)
-        ks = self.k_scale[i] if self.k_scale is not None else None
-        vs = self.v_scale[i] if self.v_scale is not None else None
-        SV.kv_append(qkv, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, slots, self.k_cache[i],
-                     self.v_cache[i], ks, vs, self.kv_dtype)
+        self._append_kv(i, qkv, slots)
         o = attn(i, qkv)
         h2 = self._linear(o, p + "wo", residual=h)
         xn2, _, _ = N.rmsnorm_fwd(h2, self.W[p + "ffn_norm"], cfg.norm_eps)
         return self._ffn(xn2, p, h2)
+
+    def _append_kv(self, i: int, qkv: torch.Tensor, slots: torch.Tensor) -> None:
+        cfg = self.cfg
+        H, KV, Dh = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
+        ks = self.k_scale[i] if self.k_scale is not None else None
+        vs = self.v_scale[i] if self.v_scale is not None else None
+        if self.page_scaled:
+            PG.page_append(qkv, H, KV, Dh, slots, self.k_cache[i], self.v_cache[i], ks, vs, self.block_size)
+        else:
+            SV.kv_append(qkv, H, KV, Dh, slots, self.k_cache[i], self.v_cache[i], ks, vs, self.kv_dtype)
+
+    def copy_pages(self, moves: List[Tuple[int, int]]) -> None:
+        """Copy KV blocks (source, destination) in every layer: forks, compaction."""
+        if moves:
+            caches = [self.k_cache, self.v_cache]
+            if self.k_scale is not None:
+                caches += [self.k_scale, self.v_scale]
+            PG.copy_pages(caches, moves, self.dummy_block + 1)
 
     def _head(self, h_last: torch.Tensor) -> torch.Tensor:
         xf, _, _ = N.rmsnorm_fwd(h_last, self.W["final_norm"], self.cfg.norm_eps)
@@ -155,6 +185,57 @@ class ModelRunner:
     # nucleus (top-p) sampling and per-request seeds run on a single-GPU kernel
     # (the nucleus threshold needs the whole vocabulary row)
     supports_top_p = True
+
+    # penalties, biases and masks need whole rows of logits
+    supports_adjust = True
+    _counts: Optional[torch.Tensor] = None
+
+    def set_counts(self, rows: List[int], histories: List[Tuple[List[int], List[int]]], table_rows: int) -> None:
+        """Write the token counts of requests (prompt, generated tokens) into their
+        rows of the table, which has table_rows rows."""
+        dev = self.device
+        if self._counts is None or self._counts.shape[0] < table_rows:
+            old = self._counts
+            self._counts = LG.token_counts(table_rows, self.cfg.vocab_size, dev)
+            if old is not None:
+                self._counts[:old.shape[0]] = old
+        tokens, offsets, prompts = [], [0], []
+        for prompt, out in histories:
+            tokens += prompt
+            tokens += out
+            offsets.append(len(tokens))
+            prompts.append(len(prompt))
+        LG.set_token_counts(self._counts, torch.tensor(rows, dtype=torch.int32, device=dev),
+                            torch.tensor(tokens, dtype=torch.int64, device=dev),
+                            torch.tensor(offsets, dtype=torch.int32, device=dev),
+                            torch.tensor(prompts, dtype=torch.int32, device=dev))
+
+    def add_counts(self, rows: List[int], tokens: torch.Tensor) -> None:
+        """Count the sampled tokens [n] (row -1: a request without penalties)."""
+        LG.add_token_counts(self._counts, torch.tensor(rows, dtype=torch.int32, device=self.device), tokens)
+
+    def adjust_logits(self, logits: torch.Tensor, rows: List[int], penalties: List[Tuple[float, float, float]],
+                      biases: List[Optional[Dict[int, float]]], allowed: List[Optional[List[int]]]) -> torch.Tensor:
+        """logits [n, vocab] changed in place: each request's penalties (row of the
+        counts table, -1 = none), biases {token: bias} and, where given, the only
+        tokens that its grammar allows."""
+        dev, V = self.device, self.cfg.vocab_size
+        counts = rows_t = pen = mask = mask_rows = None
+        if any(r >= 0 for r in rows):
+            counts, rows_t = self._counts, torch.tensor(rows, dtype=torch.int32, device=dev)
+            pen = torch.tensor(penalties, dtype=torch.float32, device=dev)
+        which = [k for k, a in enumerate(allowed) if a is not None]
+        if which:
+            bits = np.zeros((len(which), (V + 31) // 32 * 32), dtype=np.uint8)
+            at = [-1] * len(allowed)
+            for m, k in enumerate(which):
+                bits[m, np.asarray(allowed[k], dtype=np.int64)] = 1
+                at[k] = m
+            words = np.packbits(bits, axis=1, bitorder="little").view(np.int32)
+            mask = torch.from_numpy(words).to(dev)
+            mask_rows = torch.tensor(at, dtype=torch.int32, device=dev)
+        return LG.adjust_logits(logits, counts, rows_t, pen, bias=LG.logit_bias(biases, dev), mask=mask,
+                                mask_rows=mask_rows, out=logits)
 
     def sample(self, logits: torch.Tensor, temps: Optional[List[float]], seed: int,
                top_ps: Optional[List[float]] = None, row_seeds: Optional[List[int]] = None) -> torch.Tensor:
@@ -172,6 +253,10 @@ class ModelRunner:
                 torch.tensor([x & ((1 << 63) - 1) for x in row_seeds], dtype=torch.int64, device=dev)
             return SV.sample_topp(logits, t, p, seed, row_seeds=rs)
         return SV.sample(logits, t, seed)
+
+    # a chunk of up to this many rows attends to the pages themselves instead of a bf16 copy
+    # of its context
+    PAGE_ATTN_ROWS = 16
 
     # -------------------------------------------------------------- prefill
     @torch.no_grad()
@@ -196,13 +281,28 @@ class ModelRunner:
         all_slots = [torch.tensor(it.slots[:it.start + len(it.tokens)], dtype=torch.int32, device=dev)
                      for it in items]
         H, KV, Dh = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
+        bs = self.block_size
+        pages = [None] * len(items)  # (page table, length) of the chunks that attend to the pages themselves
+        if self.page_scaled:
+            for k, it in enumerate(items):
+                if it.start > 0 and len(it.tokens) <= self.PAGE_ATTN_ROWS:
+                    end = it.start + len(it.tokens)
+                    pages[k] = (torch.tensor([[s // bs for s in it.slots[:end:bs]]], dtype=torch.int32, device=dev),
+                                torch.tensor([end], dtype=torch.int32, device=dev))
 
         def attn(i, qkv):
             o = torch.empty(qkv.shape[0], H * Dh, dtype=torch.bfloat16, device=dev)
             ks = self.k_scale[i] if self.k_scale is not None else None
             vs = self.v_scale[i] if self.v_scale is not None else None
-            for it, (a, b), sl in zip(items, bounds, all_slots):
-                kv = SV.kv_gather(self.k_cache[i], self.v_cache[i], ks, vs, sl, KV, Dh, self.kv_dtype)
+            for it, (a, b), sl, pg in zip(items, bounds, all_slots, pages):
+                if pg is not None:
+                    PG.page_attention(qkv[a:b, :H * Dh], self.k_cache[i], self.v_cache[i], ks, vs, pg[0], pg[1], bs,
+                                      H, KV, Dh, q_len=b - a, max_ctx=it.start + b - a, out=o[a:b])
+                    continue
+                if self.page_scaled:
+                    kv = PG.page_gather(self.k_cache[i], self.v_cache[i], ks, vs, sl, KV, Dh, bs)
+                else:
+                    kv = SV.kv_gather(self.k_cache[i], self.v_cache[i], ks, vs, sl, KV, Dh, self.kv_dtype)
                 attention_fwd(qkv[a:b, :H * Dh], 1, b - a, H, KV, Dh, causal=True, out=o[a:b],
                               kv=kv, q_off=it.start)
             return o
@@ -256,6 +356,9 @@ class ModelRunner:
         def attn(i, qkv):
             ks = self.k_scale[i] if self.k_scale is not None else None
             vs = self.v_scale[i] if self.v_scale is not None else None
+            if self.page_scaled:
+                return PG.page_attention(qkv[:, :H * Dh], self.k_cache[i], self.v_cache[i], ks, vs, bt, ctx,
+                                         self.block_size, H, KV, Dh, max_ctx=max_ctx)
             return SV.decode_attention(qkv[:, :H * Dh], self.k_cache[i], self.v_cache[i], ks, vs, bt, ctx,
                                        self.block_size, H, KV, Dh, kv_dtype=self.kv_dtype, max_ctx=max_ctx)
 
@@ -287,6 +390,11 @@ class ModelRunner:
         ctx = torch.tensor([int(p) + 1 for p in positions], dtype=torch.int32, device=dev)
         return self._decode_body(ids_t, pos_t, slots_t, bt, ctx, int(max(positions)) + 1)
 
+    @property
+    def _pad_slot(self) -> int:
+        """Slot of a padding row: the reserved block; none where rows of a block must not meet in one call."""
+        return -1 if self.page_scaled else self.dummy_block * self.block_size
+
     def _decode_graph(self, tokens, positions, slots, block_tables) -> torch.Tensor:
         n = len(tokens)
         b = next(x for x in self.GRAPH_BUCKETS if x >= n)
@@ -302,7 +410,7 @@ class ModelRunner:
         hi[0:n] = tokens
         hi[b:b + n] = positions
         hi[2 * b:2 * b + n] = slots
-        hi[2 * b + n:3 * b] = self.dummy_block * self.block_size
+        hi[2 * b + n:3 * b] = self._pad_slot
         hi[3 * b:3 * b + n] = np.asarray(positions, dtype=np.int32) + 1
         hi[3 * b + n:4 * b] = 1
         btab = hi[4 * b:].reshape(b, mb)
@@ -326,7 +434,7 @@ class ModelRunner:
         ctx = dev_in[3 * b:4 * b]
         bt = dev_in[4 * b:].view(b, mb)
         # a valid dummy batch for warm-up and capture: every row is padding
-        host[2 * b:3 * b] = self.dummy_block * self.block_size
+        host[2 * b:3 * b] = self._pad_slot
         host[3 * b:4 * b] = 1
         host[4 * b:].view(b, mb)[:, 0] = self.dummy_block
         dev_in.copy_(host)

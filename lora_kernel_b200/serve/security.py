@@ -35,10 +35,35 @@ class ValidationError(ValueError):
 
 
 class InputValidator:
-    def __init__(self, vocab_size: int, max_prompt_tokens: int = 32768, max_new_tokens: int = 8192):
+    def __init__(self, vocab_size: int, max_prompt_tokens: int = 32768, max_new_tokens: int = 8192,
+                 adjust: bool = False):
+        """adjust: the engine changes logits (penalties, biases, allowed tokens)."""
         self.vocab_size = vocab_size
+        self.adjust = adjust
         self.max_prompt_tokens = max_prompt_tokens
         self.max_new_tokens = max_new_tokens
+
+    def _check_adjust(self, body: dict) -> None:
+        for k in ("presence_penalty", "frequency_penalty"):
+            x = body.get(k)
+            if x is not None and not (_number(x) and -2.0 <= x <= 2.0):
+                raise ValidationError(f"{k} must be in [-2, 2]")
+        x = body.get("repetition_penalty")
+        if x is not None and not (_number(x) and 0.01 <= x <= 100.0):
+            raise ValidationError("repetition_penalty must be in [0.01, 100]")
+        bias = body.get("logit_bias")
+        if bias is not None:
+            if not isinstance(bias, dict) or len(bias) > 1024:
+                raise ValidationError("logit_bias must be an object of at most 1024 token ids")
+            for k, v in bias.items():
+                if not (isinstance(k, str) and k.isascii() and k.isdigit() and len(k) < 10 and int(k) < self.vocab_size):
+                    raise ValidationError(f"logit_bias: {k!r} is not a token id in [0, {self.vocab_size})")
+                if not (_number(v) and -100.0 <= v <= 100.0):
+                    raise ValidationError("logit_bias: values must be in [-100, 100]")
+        ids = body.get("allowed_token_ids")
+        if ids is not None and not (isinstance(ids, list) and 0 < len(ids) <= self.vocab_size and all(
+                isinstance(t, int) and not isinstance(t, bool) and 0 <= t < self.vocab_size for t in ids)):
+            raise ValidationError(f"allowed_token_ids must be a non-empty list of token ids in [0, {self.vocab_size})")
 
     def check(self, ids: Sequence[int], body: dict) -> None:
         if not ids:
@@ -60,8 +85,10 @@ class InputValidator:
         n = body.get("n", 1)
         if n != 1:
             raise ValidationError("n must be 1 (one choice per request)")
+        if self.adjust:
+            self._check_adjust(body)
         for k in ("presence_penalty", "frequency_penalty"):
-            if body.get(k, 0) not in (0, 0.0, None):
+            if not self.adjust and body.get(k, 0) not in (0, 0.0, None):
                 raise ValidationError(f"{k} is not supported (use 0)")
         if body.get("logprobs") not in (None, False, 0):
             raise ValidationError("logprobs are not returned by this server")
@@ -81,6 +108,10 @@ class InputValidator:
             if not isinstance(seqs, list) or len(seqs) > 4 or \
                     not all(isinstance(x, str) and 0 < len(x) <= 256 for x in seqs):
                 raise ValidationError("stop must be a string or a list of at most 4 non-empty strings")
+
+
+def _number(x) -> bool:
+    return isinstance(x, (int, float)) and not isinstance(x, bool)
 
 
 def _luhn_ok(digits: str) -> bool:

@@ -270,7 +270,8 @@ def create_app(engine: LLMEngine, model_name: str = "lora-kernel-b200", api_keys
     tok = tokenizer or ByteTokenizer(engine.cfg.vocab_size)
     bucket = TokenBucket(rate_limit_rps, max(1.0, rate_limit_rps * 2)) if rate_limit_rps > 0 else None
     keys = set(api_keys)
-    validator = validator or InputValidator(engine.cfg.vocab_size)
+    adjust = all(getattr(getattr(e, "runner", None), "supports_adjust", False) for e in engines)
+    validator = validator or InputValidator(engine.cfg.vocab_size, adjust=adjust)
     masker = PIIMasker() if pii_filter else None
     signer = RequestSigner(signing_secret) if signing_secret else None
 
@@ -337,7 +338,16 @@ def create_app(engine: LLMEngine, model_name: str = "lora-kernel-b200", api_keys
         return SamplingParams(max_tokens=int(body.get("max_tokens", 16)),
                               temperature=float(body.get("temperature", 0.0) or 0.0),
                               top_p=float(body.get("top_p", 1.0) or 1.0), stop_token_ids=tuple(stop),
-                              stop_sequences=seqs, seed=body.get("seed"))
+                              stop_sequences=seqs, seed=body.get("seed"), **_adjustments(body))
+
+    def _adjustments(body) -> dict:
+        if not adjust:
+            return {}
+        bias = {int(k): float(v) for k, v in (body.get("logit_bias") or {}).items()}
+        return dict(repetition_penalty=float(body.get("repetition_penalty") or 1.0),
+                    frequency_penalty=float(body.get("frequency_penalty") or 0.0),
+                    presence_penalty=float(body.get("presence_penalty") or 0.0),
+                    logit_bias=bias or None, allowed_token_ids=body.get("allowed_token_ids"))
 
     async def _run(prompt, params, stream: bool, request: web.Request, chat: bool, priority: int = 0):
         loop = asyncio.get_running_loop()

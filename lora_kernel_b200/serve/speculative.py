@@ -61,6 +61,8 @@ class RunnerScorer(Scorer):
         self.max_len = max_len or runner.max_model_len
         if base_slot + self.max_len > runner.num_blocks * runner.block_size:
             raise ValueError("RunnerScorer: slot range exceeds the runner's KV cache")
+        if getattr(runner, "page_scaled", False) and base_slot % runner.block_size:
+            raise ValueError("RunnerScorer: a page-scaled cache needs a base slot at the start of a page")
         self.seq_id = seq_id
         self._len = 0
 

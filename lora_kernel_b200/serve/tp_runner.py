@@ -81,6 +81,7 @@ class TPModelRunner(ModelRunner):
 
     # each rank holds a vocabulary slice; the top-p threshold would need the whole row
     supports_top_p = False
+    supports_adjust = False  # the counts table and the masks are laid out for whole rows
 
     def __init__(self, cfg: TransformerConfig, params, comm: TPServeComm, device="cuda", **kw):
         tp = comm.tp
@@ -104,10 +105,7 @@ class TPModelRunner(ModelRunner):
         xn = self._xn if self._xn is not None else N.rmsnorm_fwd(h, self.W[p + "attn_norm"], cfg.norm_eps)[0]
         qkv = self._linear(xn, p + "wqkv")
         E.rope_(qkv, 0, cfg.num_heads + cfg.num_kv_heads, cfg.head_dim, self.rope, positions=pos)
-        ks = self.k_scale[i] if self.k_scale is not None else None
-        vs = self.v_scale[i] if self.v_scale is not None else None
-        SV.kv_append(qkv, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, slots, self.k_cache[i],
-                     self.v_cache[i], ks, vs, self.kv_dtype)
+        self._append_kv(i, qkv, slots)
         o = attn(i, qkv)
         M = h.shape[0]
         self._row_parallel(o, p + "wo", c.partial(M))
