@@ -1197,10 +1197,13 @@ void page_append(torch::Tensor qkv, int64_t Hq, int64_t Hkv, int64_t Dh, torch::
   check(lk_page_append(&d, stream()));
 }
 
-void page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale, torch::Tensor v_scale,
-                 torch::Tensor slots, int64_t Hkv, int64_t Dh, int64_t page, torch::Tensor out, torch::Tensor status) {
-  const c10::cuda::CUDAGuard g(out.device());
+torch::Tensor page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale, torch::Tensor v_scale,
+                          torch::Tensor slots, int64_t Hkv, int64_t Dh, int64_t page,
+                          c10::optional<torch::Tensor> out_opt, torch::Tensor status) {
+  const c10::cuda::CUDAGuard g(k_cache.device());
   need_contig(slots, "slots", torch::kInt32);
+  torch::Tensor out = out_opt.has_value() ? *out_opt
+                                          : torch::empty({slots.numel(), 2 * Hkv * Dh}, k_scale.options().dtype(torch::kBFloat16));
   need(out, "out", torch::kBFloat16);
   TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == slots.numel() && out.size(1) == 2 * Hkv * Dh,
               "page_gather: out must be row-major [n, 2 * Hkv * Dh]");
@@ -1217,6 +1220,7 @@ void page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_s
   d.out = out.data_ptr(); d.ldo = out.stride(0);
   d.status = status.data_ptr<int>();
   check(lk_page_gather(&d, stream()));
+  return out;
 }
 
 torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor k_scale,

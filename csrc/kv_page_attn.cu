@@ -44,10 +44,16 @@ namespace lk {
 #ifndef PA_STAGES
 #define PA_STAGES 2
 #endif
+#ifndef PA_B2
+#define PA_B2 3
+#endif
+#ifndef PA_W
+#define PA_W 4
+#endif
 #ifndef PA_BLOCKS
 #define PA_BLOCKS 3
 #endif
-constexpr int PA_WARPS = 4;
+constexpr int PA_WARPS = PA_W;
 constexpr int PA_UNIT = 32;        // tokens a warp takes at a time (two M = 16 tiles)
 constexpr float PA_LOW = -3.0e38f;  // reference before the first token
 constexpr float PA_TOP = 14.f, PA_AIM = 7.f;
@@ -148,7 +154,7 @@ __device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int se
 
 // Grid: split fastest, then KV head, row tile (8 * NT query rows), sequence.
 template <int KV, int DH, int NT>
-__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_attn_kernel(LkPageAttnDesc d, int tiles, FastDiv pages) {
+__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : (DH == 64 ? PA_B2 : 2)) page_attn_kernel(LkPageAttnDesc d, int tiles, FastDiv pages) {
   const int nsplit = d.nsplit;
   using R = PaRing<DH>;
   constexpr int ROWS = 8 * NT, CH = DH / 64, MT = DH / 16;
@@ -426,7 +432,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
   cp_wait<0>();
   __syncthreads();
 
-  // merge the warps: [warp][row][DH + 3] floats over the ring
+  // merge the warps: [warp][row][DH + 4] floats over the ring, a warp a row
   float* part = reinterpret_cast<float*>(sm);
   constexpr int PITCH = DH + 4;
 #pragma unroll
@@ -442,77 +448,112 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? PA_BLOCKS : 2) page_a
         row[r * (DH / 8) + 2 * j] = acc[n][j][q];
         row[r * (DH / 8) + 2 * j + 1] = acc[n][j][2 + q];
       }
-      if (r == 0) row[DH] = ms[n][q], row[DH + 1] = mw[n][q], row[DH + 2] = x;
+      if (r == 0) *reinterpret_cast<float4*>(row + DH) = make_float4(ms[n][q], mw[n][q], x, 0.f);
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < ROWS * DH; i += 32 * PA_WARPS) {
-    const int rl = i / DH, dim = i % DH, row = tile * ROWS + rl;
+  for (int rl = warp; rl < ROWS; rl += PA_WARPS) {
+    const int row = tile * ROWS + rl;
     if (row >= rows) break;
     const float* x = part + rl * PITCH;
-    float MS = PA_LOW, MW = PA_LOW, L = 0.f, O = 0.f;
+    float4 ml[PA_WARPS];
+    float MS = PA_LOW, MW = PA_LOW, L = 0.f, o[DH / 32];
 #pragma unroll
     for (int w = 0; w < PA_WARPS; ++w) {
-      MS = fmaxf(MS, x[w * ROWS * PITCH + DH]);
-      MW = fmaxf(MW, x[w * ROWS * PITCH + DH + 1]);
+      ml[w] = *reinterpret_cast<const float4*>(x + w * ROWS * PITCH + DH);
+      MS = fmaxf(MS, ml[w].x);
+      MW = fmaxf(MW, ml[w].y);
     }
 #pragma unroll
+    for (int i = 0; i < DH / 32; ++i) o[i] = 0.f;
+#pragma unroll
     for (int w = 0; w < PA_WARPS; ++w) {
-      const float* y = x + w * ROWS * PITCH;
-      L += y[DH + 2] * fast_exp2(y[DH] - MS);
-      O += y[dim] * fast_exp2(y[DH + 1] - MW);
+      L += ml[w].z * fast_exp2(ml[w].x - MS);
+      const float f = fast_exp2(ml[w].y - MW);
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) o[i] = fmaf(x[w * ROWS * PITCH + i * 32 + lane], f, o[i]);
     }
     const int64_t grow = (int64_t)seq * d.q_len + row / group;
     const int head = h * group + row % group;
     if (nsplit == 1) {
-      O *= fast_exp2(MW - MS);
-      ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + dim] = __float2bfloat16(L == 0.f ? 0.f : O / L);
+      const float f = L == 0.f ? 0.f : fast_exp2(MW - MS) / L;
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + i * 32 + lane] = __float2bfloat16(o[i] * f);
     } else {
       const int64_t at = (grow * d.Hq + head) * nsplit + split;
-      d.part_o[at * DH + dim] = O;
-      if (dim == 0) *reinterpret_cast<float4*>(d.part_ml + at * 4) = make_float4(MS, MW, L, 0.f);
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) d.part_o[at * DH + i * 32 + lane] = o[i];
+      if (lane == 0) *reinterpret_cast<float4*>(d.part_ml + at * 4) = make_float4(MS, MW, L, 0.f);
     }
   }
 }
 
-// Joins the parts of a (row, head): one warp each, in the order of the parts.
+// Joins the parts of a (row, head), a block each: every warp finds the references and
+// the sum from all parts (a lane per part), then takes every fourth part's output, eight
+// of them on their way at once.  Sums are in a fixed order.  (A warp alone, part after
+// part, took 14 us for 18 parts and 24 us for 37.)
+constexpr int JOIN_WARPS = 4;
+
 template <int DH>
-__global__ void page_attn_join_kernel(LkPageAttnDesc d, int tile_rows, int nsplit) {
-  const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  cudaGridDependencySynchronize();  // the parts are written
-  if (w >= (int64_t)d.num_seqs * d.q_len * d.Hq) return;
+__global__ void __launch_bounds__(32 * JOIN_WARPS) page_attn_join_kernel(LkPageAttnDesc d, int tile_rows, int nsplit) {
+  __shared__ float so[JOIN_WARPS][DH];
+  const int64_t w = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t grow = w / d.Hq;
   const int head = (int)(w % d.Hq), group = d.Hq / d.Hkv;
   const int row = (int)(grow % d.q_len) * group + head % group;
   const int last = min(group * d.q_len, (row / tile_rows + 1) * tile_rows) - 1;
   const PaSpan sp = page_attn_span(d, (int)(grow / d.q_len), last, group);
   const int used = max(1, (sp.units + sp.per - 1) / sp.per);
+  cudaGridDependencySynchronize();  // the parts are written
   const float4* ml = reinterpret_cast<const float4*>(d.part_ml) + w * nsplit;
+  const float* po = d.part_o + w * nsplit * DH + lane;
   float MS = PA_LOW, MW = PA_LOW, L = 0.f, o[DH / 32];
-  for (int s = 0; s < used; ++s) {
-    MS = fmaxf(MS, ml[s].x);
-    MW = fmaxf(MW, ml[s].y);
+  for (int s = lane; s < used; s += 32) {
+    const float4 x = ml[s];
+    MS = fmaxf(MS, x.x);
+    MW = fmaxf(MW, x.y);
   }
+  MS = warp_max(MS);
+  MW = warp_max(MW);
 #pragma unroll
   for (int i = 0; i < DH / 32; ++i) o[i] = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const float4 x = ml[s];
+  for (int base = 0; base < used; base += 32) {
+    const float4 x = base + lane < used ? ml[base + lane] : make_float4(PA_LOW, PA_LOW, 0.f, 0.f);
     L += x.z * fast_exp2(x.x - MS);
-    const float f = fast_exp2(x.y - MW);
+    const float f = base + lane < used ? fast_exp2(x.y - MW) : 0.f;
+    float v[32 / JOIN_WARPS][DH / 32];
 #pragma unroll
-    for (int i = 0; i < DH / 32; ++i) o[i] += d.part_o[(w * nsplit + s) * DH + i * 32 + lane] * f;
+    for (int k = 0; k < 32 / JOIN_WARPS; ++k) {
+      const int s = base + warp + JOIN_WARPS * k;
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) v[k][i] = s < used ? po[(int64_t)s * DH + i * 32] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 32 / JOIN_WARPS; ++k) {
+      const float g = __shfl_sync(0xffffffffu, f, warp + JOIN_WARPS * k);
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) o[i] = fmaf(v[k][i], g, o[i]);
+    }
   }
-  const float f = fast_exp2(MW - MS);
+  L = warp_sum(L);
 #pragma unroll
-  for (int i = 0; i < DH / 32; ++i)
-    ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + i * 32 + lane] = __float2bfloat16(L == 0.f ? 0.f : o[i] * f / L);
+  for (int i = 0; i < DH / 32; ++i) so[warp][i * 32 + lane] = o[i];
+  __syncthreads();
+  const float f = fast_exp2(MW - MS);
+  for (int c = threadIdx.x; c < DH; c += 32 * JOIN_WARPS) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < JOIN_WARPS; ++k) x += so[k][c];
+    ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + c] = __float2bfloat16(L == 0.f ? 0.f : x * f / L);
+  }
 }
 
 template <int KV, int DH, int NT>
 static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
   const int rows = d.Hq / d.Hkv * d.q_len, tiles = cdiv(rows, 8 * NT);
   const int64_t blocks = (int64_t)d.num_seqs * d.Hkv * tiles * d.nsplit;
-  LK_REQUIRE(blocks < (1ll << 31), "page_attention: too many rows in one call");
+  LK_REQUIRE(blocks < (1ll << 31) && (int64_t)d.num_seqs * d.q_len * d.Hq < (1ll << 31),
+             "page_attention: too many rows in one call");
   constexpr int merge = PA_WARPS * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
   constexpr int smem = ring > merge ? ring : merge;
   auto k = page_attn_kernel<KV, DH, NT>;
@@ -528,12 +569,12 @@ static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
   k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, tiles, FastDiv(d.page));
   if (check_launch("page_attention")) return -1;
   if (d.nsplit == 1) return 0;
-  const int64_t warps = (int64_t)d.num_seqs * d.q_len * d.Hq;
+  const int64_t joins = (int64_t)d.num_seqs * d.q_len * d.Hq;
   // launched while the parts still run (its blocks wait for them in the launch order of
   // the stream): the launch's own latency is not waited for
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(cdiv(warps * 32, 128));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)joins);
+  cfg.blockDim = dim3(32 * JOIN_WARPS);
   cfg.stream = s;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -558,7 +599,7 @@ using namespace lk;
 // (256 sequences: 190 us uncut, 206 in halves, 227 in quarters).
 extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units) {
   const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
-  const int sms = num_sms(), most = std::max(1, cdiv(max_ctx, 256));
+  const int sms = num_sms(), most = max_ctx <= 768 ? 1 : cdiv(max_ctx, 256);  // the join's launch costs 3 us
   int best = 1;
   double least = 1e30;
   for (int k = 0; k <= (rows <= 8 ? 3 : 2); ++k) {

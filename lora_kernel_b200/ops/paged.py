@@ -43,10 +43,7 @@ def page_gather(k_cache, v_cache, k_scale, v_scale, slots: torch.Tensor, Hkv: in
     """The cached keys and values at `slots` (int32 [n]) as bf16 rows [n, 2 * Hkv * Dh]
     (exact: a code times a power of two), keys first."""
     require_device(k_cache)
-    if out is None:
-        out = torch.empty(slots.numel(), 2 * Hkv * Dh, dtype=torch.bfloat16, device=k_cache.device)
-    C().page_gather(k_cache, v_cache, k_scale, v_scale, slots, Hkv, Dh, page, out, status(out.device))
-    return out
+    return C().page_gather(k_cache, v_cache, k_scale, v_scale, slots, Hkv, Dh, page, out, status(k_cache.device))
 
 
 def page_attention(q: torch.Tensor, k_cache, v_cache, k_scale, v_scale, block_tables: torch.Tensor,
