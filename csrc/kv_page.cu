@@ -30,7 +30,7 @@ namespace lk {
 // Bound by HBM for a prompt (6 bytes a value with the codes written: 8190 rows of 8
 // heads x 128 in 14 us), by the chain slot -> row -> maximum -> store for a token
 // per sequence.  A block's warps look for runs that start in its `window` rows: 1 row
-// where there are few (every run on a block of its own), 8 for prompts, where
+// where there are few (every run on a block of its own), 16 for prompts, where
 // 15 of 16 rows start none and their blocks would be empty.
 
 // 8 bf16 -> 8 codes.  CHECK: some of them are not finite (infinities saturate, NaN -> 0).
@@ -130,7 +130,7 @@ __device__ void append_run(const LkPageAppendDesc& d, int t, int rows, int slot,
 
 // grid (windows of rows, groups of 8 (head, K|V) pairs)
 template <int KV, int DH>
-__global__ void __launch_bounds__(256) page_append_kernel(LkPageAppendDesc d, int window) {
+__global__ void __launch_bounds__(256, 4) page_append_kernel(LkPageAppendDesc d, int window) {
   const int item = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (item >= 2 * d.Hkv) return;
   // lane l looks at row t0 - 1 + l: which rows continue the row before them
@@ -165,16 +165,15 @@ __global__ void __launch_bounds__(256) page_append_kernel(LkPageAppendDesc d, in
 }
 
 // ---------------------------------------------------------------- gather
-// A thread takes 16 codes of a token's keys and the same 16 of its values (the heads
-// of a slot lie side by side in the cache and in the output alike): two 16-byte loads,
-// 32 + 32 bytes written.  Bound by HBM: 3 bytes a value.
+// A thread takes 8 codes of a token's keys and the same 8 of its values (the heads of a
+// slot lie side by side in the cache and in the output alike): two 8-byte loads, two
+// 16-byte stores, a warp's stores in one piece.  Bound by HBM: 3 bytes a value.
 template <int KV>
-__device__ __forceinline__ void widen16(const uint8_t* src, float scale, __nv_bfloat16* dst) {
-  const uint4 c = *reinterpret_cast<const uint4*>(src);
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  uint32_t o[8];
+__device__ __forceinline__ uint4 widen8(uint2 c, float scale) {
+  const uint32_t w[2] = {c.x, c.y};
+  uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     float a, b;
     const uint32_t two = w[i / 2] >> (16 * (i & 1));
     if constexpr (KV == 1) {
@@ -186,28 +185,29 @@ __device__ __forceinline__ void widen16(const uint8_t* src, float scale, __nv_bf
     }
     o[i] = pack_bf16x2(a * scale, b * scale);
   }
-  reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 template <int KV>
 __global__ void __launch_bounds__(256) page_gather_kernel(LkPageGatherDesc d, int total, FastDiv per_row, FastDiv page) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= total) return;
-  const int t = per_row.div(i), at = (i - t * per_row.d) * 16;
-  const int h = at / d.Dh, width = d.Hkv * d.Dh;
+  const int t = per_row.div(i), at = (i - t * per_row.d) * 8;
+  const int h = at >> (d.Dh == 64 ? 6 : 7), width = d.Hkv * d.Dh;
   const int slot = d.slots[t];
-  __nv_bfloat16* out = (__nv_bfloat16*)d.out + (int64_t)t * d.ldo + at;
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
   if (slot < 0 || slot >= d.num_slots) {
     if (d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
-    const uint4 z = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) reinterpret_cast<uint4*>(out)[k] = z, reinterpret_cast<uint4*>(out + width)[k] = z;
-    return;
+  } else {
+    const int64_t sc = (int64_t)page.div(slot) * d.Hkv + h, from = (int64_t)slot * width + at;
+    const uint2 kc = *reinterpret_cast<const uint2*>((const uint8_t*)d.k_cache + from);
+    const uint2 vc = *reinterpret_cast<const uint2*>((const uint8_t*)d.v_cache + from);
+    k = widen8<KV>(kc, d.k_scale[sc]);
+    v = widen8<KV>(vc, d.v_scale[sc]);
   }
-  const int64_t sc = (int64_t)page.div(slot) * d.Hkv + h, from = (int64_t)slot * width + at;
-  widen16<KV>((const uint8_t*)d.k_cache + from, d.k_scale[sc], out);
-  widen16<KV>((const uint8_t*)d.v_cache + from, d.v_scale[sc], out + width);
+  __nv_bfloat16* out = (__nv_bfloat16*)d.out + (int64_t)t * d.ldo + at;
+  *reinterpret_cast<uint4*>(out) = k;
+  *reinterpret_cast<uint4*>(out + width) = v;
 }
 
 // ---------------------------------------------------------------- page copies
@@ -253,7 +253,7 @@ extern "C" int lk_page_append(const LkPageAppendDesc* d, cudaStream_t s) {
   LK_REQUIRE(d->Dh == 64 || d->Dh == 128, "page_append: head_dim must be 64 or 128");
   if (d->T == 0 || d->Hkv == 0) return 0;
   LK_REQUIRE(d->Hkv <= 4 * 65535, "page_append: too many heads");
-  const int window = d->T <= 1024 ? 1 : 8;
+  const int window = d->T <= 1024 ? 1 : 16;
   const dim3 grid(cdiv(d->T, window), cdiv(2 * d->Hkv, 8));
   if (d->kv_dtype == 1)
     d->Dh == 64 ? page_append_kernel<1, 64><<<grid, 256, 0, s>>>(*d, window) : page_append_kernel<1, 128><<<grid, 256, 0, s>>>(*d, window);
@@ -263,7 +263,7 @@ extern "C" int lk_page_append(const LkPageAppendDesc* d, cudaStream_t s) {
 }
 
 extern "C" int lk_page_gather(const LkPageGatherDesc* d, cudaStream_t s) {
-  const int per_row = d->Hkv * d->Dh / 16;
+  const int per_row = d->Hkv * d->Dh / 8;
   const int64_t total = (int64_t)d->n * per_row;
   if (total == 0) return 0;
   LK_REQUIRE(total < (1ll << 31), "page_gather: too many rows in one call");
