@@ -42,7 +42,7 @@ struct AdjGroup {
 // column: the logits stay packed, and only pairs of columns with a count or a bias are
 // taken apart (1 % of the columns are seen or biased in a request of some thousand
 // tokens: 40 % of a warp's pairs).  256 rows of 128256 with 300 biases each and masks
-// in 43.5 us, 35 without biases (torch.add of the logits and the counts: 31); 1 or 4 groups,
+// in 38.2 us, 35 without biases (torch.add of the logits and the counts: 31); 1 or 4 groups,
 // 5 blocks an SM and blocks of 512 are 2-15 us slower.
 // VEC: every row of every table starts on 16 bytes; a thread takes 8 neighbouring
 // columns at a time.  Otherwise (an odd vocabulary without a padded pitch) its 8 lie a
@@ -109,19 +109,34 @@ __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2)
 
   int any = 0;  // a bias falls into this span
   if (b0 < b1) {
+    // ids and values of a thread's first two biases are asked for together and at once:
+    // the block lives as long as its longest chain of loads
+    constexpr int FIRST = 2;
+    int id[FIRST];
+    float value[FIRST];
+#pragma unroll
+    for (int k = 0; k < FIRST; ++k) {
+      const int j = b0 + tid + k * ADJ_THREADS;
+      id[k] = j < b1 ? d.bias_ids[j] : v0;
+      value[k] = j < b1 ? d.bias_values[j] : 0.f;
+    }
     constexpr int words = G * (ADJ_STEP + ADJ_STEP / 32) / 4;
     for (int j = tid; j < words; j += ADJ_THREADS) reinterpret_cast<float4*>(extra)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();
-    for (int j = b0 + tid; j < b1; j += ADJ_THREADS) {
-      const int id = d.bias_ids[j], at = id - v0;
+    auto add = [&](int token, float x) {
+      const int at = token - v0;
       if ((unsigned)at < (unsigned)n) {
-        atomicAdd(&extra[at], d.bias_values[j]);
+        atomicAdd(&extra[at], x);
         atomicOr(&biased[at / 32], 1u << (at & 31));
         any = 1;
-      } else if (blockIdx.x == 0 && (unsigned)id >= (unsigned)d.vocab && d.status) {
+      } else if (blockIdx.x == 0 && (unsigned)token >= (unsigned)d.vocab && d.status) {
         atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
       }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < FIRST; ++k)
+      if (b0 + tid + k * ADJ_THREADS < b1) add(id[k], value[k]);
+    for (int j = b0 + tid + FIRST * ADJ_THREADS; j < b1; j += ADJ_THREADS) add(d.bias_ids[j], d.bias_values[j]);
     any = __syncthreads_or(any);
   }
 
