@@ -139,48 +139,66 @@ struct PaSpan {
   int ctx, end, units, per;
 };
 
-__device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int seq, int last_row, int group) {
+__device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int ctx, int last_token) {
   PaSpan s;
-  s.ctx = (int)min((int64_t)max(d.ctx_lens[seq], 0), (int64_t)d.max_pages * d.page);
-  s.end = max(0, s.ctx - d.q_len + last_row / group + 1);
+  s.ctx = (int)min((int64_t)max(ctx, 0), (int64_t)d.max_pages * d.page);
+  s.end = max(0, s.ctx - d.q_len + last_token + 1);
   s.units = (s.end + PA_UNIT - 1) / PA_UNIT;
   s.per = max((s.units + d.nsplit - 1) / d.nsplit, d.min_units);
   return s;
 }
 
+struct PaDivs {
+  FastDiv nsplit, heads, tiles, group, page;
+};
+
 // Grid: split fastest, then KV head, row tile (8 * NT query rows), sequence.
 template <int KV, int DH, int NT>
-__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) page_attn_kernel(LkPageAttnDesc d, int tiles, FastDiv pages) {
-  const int nsplit = d.nsplit;
+__global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : (DH == 64 ? 3 : 2)) page_attn_kernel(LkPageAttnDesc d, PaDivs by) {
+  const int nsplit = d.nsplit, tiles = by.tiles.d;
   using R = PaRing<DH>;
   constexpr int ROWS = 8 * NT, CH = DH / 64, MT = DH / 16;
   extern __shared__ __align__(16) uint8_t sm[];
-  const int split = blockIdx.x % nsplit;
-  int b = blockIdx.x / nsplit;
-  const int h = b % d.Hkv;
-  b /= d.Hkv;
-  const int tile = b % tiles, seq = b / tiles;
-  const int group = d.Hq / d.Hkv, rows = group * d.q_len;
+  // divisions by multiplication: a dozen of them are a good part of a short block's time
+  int b = by.nsplit.div(blockIdx.x);
+  const int split = blockIdx.x - b * nsplit;
+  int h = b;
+  b = by.heads.div(b);
+  h -= b * d.Hkv;
+  const int seq = by.tiles.div(b), tile = b - seq * tiles;
+  const int group = by.group.d, rows = group * d.q_len;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const PaSpan sp = page_attn_span(d, seq, min(rows, (tile + 1) * ROWS) - 1, group);
-  if (threadIdx.x == 0 && d.ctx_lens[seq] > (int64_t)d.max_pages * d.page && d.status)
-    atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
+  const int ctx = d.ctx_lens[seq];
+  const int* table = d.tables + (int64_t)seq * d.max_pages;
+  auto page_of = [&](int u) {  // of this lane's token of unit u; anything beyond the context is not used
+    const int i = by.page.div(u * PA_UNIT + lane);
+    return i < d.max_pages ? table[i] : 0;
+  };
+  // an uncut context begins at unit `warp` whatever its length: its pages are looked up
+  // while the length is on its way
+  int pg[PA_STAGES + 1];
+  if (nsplit == 1) {
+#pragma unroll
+    for (int s = 0; s <= PA_STAGES; ++s) pg[s] = page_of(warp + s * PA_WARPS);
+  }
+  const PaSpan sp = page_attn_span(d, ctx, by.group.div(min(rows, (tile + 1) * ROWS) - 1));
+  if (threadIdx.x == 0 && ctx > (int64_t)d.max_pages * d.page && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
   const int u_end = min(sp.units, (split + 1) * sp.per);
   cudaTriggerProgrammaticLaunchCompletion();  // the join may be brought up; it waits for all of this grid
   if (split > 0 && split * sp.per >= sp.units) return;
+  int u = split * sp.per + warp;
+  if (nsplit > 1) {
+#pragma unroll
+    for (int s = 0; s <= PA_STAGES; ++s) pg[s] = page_of(u + s * PA_WARPS);
+  }
 
   // where this lane copies from, and this warp's ring
   const uint32_t tok_stride = (uint32_t)d.Hkv * DH;
   const uint8_t* kbase = (const uint8_t*)d.k_cache + h * DH + lane % R::LANES * 16;
   const uint8_t* vbase = (const uint8_t*)d.v_cache + h * DH + lane % R::LANES * 16;
-  const int* table = d.tables + (int64_t)seq * d.max_pages;
   uint8_t* ring = sm + warp * R::WARP;
   const uint32_t ring_u = smem_u32(ring);
 
-  auto page_of = [&](int u) {
-    const int t = u * PA_UNIT + lane;
-    return u < u_end && t < sp.end ? table[pages.div(t)] : 0;
-  };
   // the unit's copies: this lane looks up token `lane`, then copies 16 bytes of its share
   // of the rows (8 lanes a 128-byte line, so that a request is a whole line); its token's
   // scales go to registers and into the stage when the unit's turn comes
@@ -190,7 +208,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
       const bool there = t < sp.end, ok = there && (unsigned)pg < (unsigned)d.num_pages;
       const unsigned valid = __ballot_sync(0xffffffffu, ok);
       const uint32_t st = ring_u + stage * R::STAGE;
-      const uint32_t slot = ok ? pg * d.page + (t - pages.div(t) * d.page) : 0;
+      const uint32_t slot = ok ? pg * d.page + (t - by.page.div(t) * d.page) : 0;
       const int64_t sc = ok ? (int64_t)pg * d.Hkv + h : 0;
       scales = make_float2(d.k_scale[sc], d.v_scale[sc]);
       if (lane == 0) asm volatile("st.shared.u32 [%0+%1], %2;" ::"r"(st), "n"(R::MASK), "r"(valid) : "memory");
@@ -213,12 +231,6 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
     cp_commit();
   };
 
-  int u = split * sp.per + warp;
-  float2 scales[R::STAGES];  // of the units in flight, the next one first
-#pragma unroll
-  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, page_of(u + s * PA_WARPS), scales[s]);
-  int pg = page_of(u + R::STAGES * PA_WARPS);
-
   // query fragments: column r of each tile, the dims of this lane's key bytes, times
   // a power of two that brings the tile's largest value to [2^14, 2^15): f16 then
   // holds a bf16 value exactly down to 2^-31 of it, and 2^-39 of it is the rounding
@@ -232,9 +244,9 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
 #pragma unroll
     for (int i = 0; i < 8 * CH; ++i) w[i / 2][i % 2] = 0;
     if (row < rows) {
-      const uint4* p = reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.q +
-                                                      ((int64_t)seq * d.q_len + row / group) * d.ldq +
-                                                      (h * group + row % group) * DH);
+      const int token = by.group.div(row);
+      const uint4* p = reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.q + ((int64_t)seq * d.q_len + token) * d.ldq +
+                                                      (h * group + row - token * group) * DH);
 #pragma unroll
       for (int k = 0; k < CH; ++k)
 #pragma unroll
@@ -243,13 +255,21 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
           w[k * 4 + i * 2][0] = v.x, w[k * 4 + i * 2][1] = v.y, w[k * 4 + i * 2 + 1][0] = v.z, w[k * 4 + i * 2 + 1][1] = v.w;
         }
     }
+  }
+
+  float2 scales[R::STAGES];  // of the units in flight, the next one first
+#pragma unroll
+  for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, pg[s], scales[s]);
+  int pg_next = pg[R::STAGES];
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int i = 0; i < 8 * CH; ++i) {
-      const float2 f = unpack_bf16x2(w[i / 2][i % 2]);
+      const float2 f = unpack_bf16x2(qf[n][i / 2][i % 2]);
       if (fabsf(f.x) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.x));
       if (fabsf(f.y) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.y));
     }
-  }
   const int e = max((int)(__float_as_uint(warp_max(amax)) >> 23) - 127 - 14, -112);
   const float down = __uint_as_float((uint32_t)(127 - e) << 23);
   const float qfac = __uint_as_float((uint32_t)(127 + e) << 23) * (d.scale * 1.4426950408889634f);
@@ -266,10 +286,10 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int col = tile * ROWS + n * 8 + 2 * c + i;
-      lim[n][i] = col < rows ? sp.ctx - d.q_len + col / group + 1 : sp.end;
+      lim[n][i] = col < rows ? sp.ctx - d.q_len + by.group.div(col) + 1 : sp.end;
     }
   }
-  const int open = sp.ctx - d.q_len + tile * ROWS / group + 1;  // tokens that every query of the tile sees
+  const int open = sp.ctx - d.q_len + by.group.div(tile * ROWS) + 1;  // tokens that every query of the tile sees
 
   float acc[NT][MT][4], ms[NT][2], mw[NT][2], l[NT][2];
 #pragma unroll
@@ -421,8 +441,8 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
     __syncwarp();  // every lane is done with the stage
 #pragma unroll
     for (int i = 0; i + 1 < R::STAGES; ++i) scales[i] = scales[i + 1];
-    issue(u + R::STAGES * PA_WARPS, stage, pg, scales[R::STAGES - 1]);
-    pg = page_of(u + (R::STAGES + 1) * PA_WARPS);
+    issue(u + R::STAGES * PA_WARPS, stage, pg_next, scales[R::STAGES - 1]);
+    pg_next = page_of(u + (R::STAGES + 1) * PA_WARPS);
     stage = stage + 1 == R::STAGES ? 0 : stage + 1;
   }
   cp_wait<0>();
@@ -468,8 +488,8 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 || DH == 64 ? 3 : 2) pa
 #pragma unroll
       for (int i = 0; i < DH / 32; ++i) o[i] = fmaf(x[w * ROWS * PITCH + i * 32 + lane], f, o[i]);
     }
-    const int64_t grow = (int64_t)seq * d.q_len + row / group;
-    const int head = h * group + row % group;
+    const int token = by.group.div(row), head = h * group + row - token * group;
+    const int64_t grow = (int64_t)seq * d.q_len + token;
     if (nsplit == 1) {
       const float f = L == 0.f ? 0.f : fast_exp2(MW - MS) / L;
 #pragma unroll
@@ -498,7 +518,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) page_attn_join_kernel(LkPageA
   const int head = (int)(w % d.Hq), group = d.Hq / d.Hkv;
   const int row = (int)(grow % d.q_len) * group + head % group;
   const int last = min(group * d.q_len, (row / tile_rows + 1) * tile_rows) - 1;
-  const PaSpan sp = page_attn_span(d, (int)(grow / d.q_len), last, group);
+  const PaSpan sp = page_attn_span(d, d.ctx_lens[grow / d.q_len], last / group);
   const int used = max(1, (sp.units + sp.per - 1) / sp.per);
   cudaGridDependencySynchronize();  // the parts are written
   const float4* ml = reinterpret_cast<const float4*>(d.part_ml) + w * nsplit;
@@ -562,7 +582,8 @@ static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
       return check_launch("page_attention: shared memory");
     ready.fetch_or(bit);
   }
-  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(d, tiles, FastDiv(d.page));
+  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(
+      d, PaDivs{FastDiv(d.nsplit), FastDiv(d.Hkv), FastDiv(tiles), FastDiv(d.Hq / d.Hkv), FastDiv(d.page)});
   if (check_launch("page_attention")) return -1;
   if (d.nsplit == 1) return 0;
   const int64_t joins = (int64_t)d.num_seqs * d.q_len * d.Hq;
