@@ -33,11 +33,12 @@
 // ones whichever the query looks at.  The softmax sum is kept in fp32 apart.
 //
 // Measured: 256 sequences of up to 4096 tokens (32 / 8 heads of 128, e4m3, 1084 MB)
-// 187-198 us, 84-88 % of the HBM copy rate; two of 100003 tokens 66 us (77 %, join
-// included); int8 codes take two instructions more a pair: 209 us.  A warp's 620
-// instructions per 32 tokens and their dependences bound it where rows are few: 24
-// sequences of up to 2047 tokens 15 us with one query each, 25 with five (8 heads of
-// 64 a group).
+// 185-197 us, 84-89 % of the HBM copy rate; two of 100003 tokens 64-66 us (77-79 %,
+// join included); int8 codes take two instructions more a pair: 200 us.  A block costs
+// 3.5 us beside its tokens (length and pages, first data, merge), which is what the full
+// batch lacks, and at head_dim 64 more (67 us for a floor of 42).  Where rows are few, a
+// warp's 620 instructions per 32 tokens and their dependences bound it: 24 sequences of
+// up to 2047 tokens with five queries each (40 rows, 8 / 1 heads of 64) 23 us.
 #include <algorithm>
 #include <utility>
 
@@ -608,23 +609,30 @@ using namespace lk;
 
 // Into how many parts a context may be cut, and the least units of a part, from the
 // longest context that the host expects (each block cuts its sequence's own length).
-// The SM with the most blocks decides: k blocks each of a part, beside which a block
-// costs what 150 tokens cost (2.3 us); with k = 1 an SM reaches 60 % of the rate that it
-// has with 2 or 3 (two contexts of 100003 tokens: 105 us with 128 blocks, 72 with 288,
-// 74 with 432, 79 with 368, which leave some SMs 3 and some 2).  Where the sequences
-// alone fill the GPU only contexts over 4096 are cut, so that one does not run on alone
-// (256 sequences: 190 us uncut, 206 in halves, 227 in quarters).
+// The estimate, in tokens that an SM takes at its full rate:
+//   a part and what a block costs beside it (150 tokens: 2.3 us shared by the blocks of
+//   an SM), times the parts of an SM - half of the time the fullest SM decides (equal
+//   lengths), half the mean, of lengths that are 0.6 of the longest;
+//   but no less than the longest part alone, at the 60 % of the rate that one block reaches;
+//   300 more for a second launch.
+// Measured (us; uncut, chosen, best): 2 contexts of 100003: 731, 64 (18 parts), 64; 8
+// sequences of up to 4096 (8 KV heads of 128): 39, 19, 17; 32: 46, 40, 40; 256: 186, uncut.
+// Beyond what fills the GPU only contexts over 4096 are cut, so that one does not run on
+// alone.
 extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units) {
   const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
-  const int sms = num_sms(), most = max_ctx <= 768 ? 1 : cdiv(max_ctx, 256);  // the join's launch costs 3 us
+  const int sms = num_sms(), most = max_ctx <= 768 ? 1 : cdiv(max_ctx, 256);
+  const int full = (int)std::min<int64_t>(most, 3 * (int64_t)sms / blocks + 1), step = std::max(1, full / 32);
   int best = 1;
   double least = 1e30;
-  for (int k = 0; k <= (rows <= 8 ? 3 : 2); ++k) {
-    const int ns = (int)std::min<int64_t>(most, std::max<int64_t>(1, (int64_t)k * sms / blocks));
-    const int64_t load = (blocks * ns + sms - 1) / sms;
-    const double cost = load * ((double)max_ctx / ns + 150) * (load == 1 ? 1.6 : 1.0);
-    if (cost < least) least = cost, best = ns;
-  }
+  auto consider = [&](int64_t ns) {
+    if (ns < 1 || ns > full) return;
+    const double part = (double)max_ctx / ns + 150, mean = 0.6 * blocks * ns / sms;
+    const double cost = std::max(part * 0.5 * ((double)((blocks * ns + sms - 1) / sms) + mean), part / 0.6) + (ns > 1 ? 300 : 0);
+    if (cost < least) least = cost, best = (int)ns;
+  };
+  for (int ns = 1; ns <= full; ns += step) consider(ns);
+  for (int k = 1; k <= 3; ++k) consider((int64_t)k * sms / blocks);
   *nsplit = best > 1 ? best : std::max(1, cdiv(max_ctx, 4096));
   *min_units = best > 1 ? 256 / PA_UNIT : 4096 / PA_UNIT;
 }
