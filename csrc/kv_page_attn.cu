@@ -182,6 +182,30 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
 #pragma unroll
     for (int s = 0; s <= PA_STAGES; ++s) pg[s] = page_of(warp + s * PA_WARPS);
   }
+  // query fragments: column r of each tile, the dims of this lane's key bytes, times
+  // a power of two that brings the tile's largest value to [2^14, 2^15): f16 then
+  // holds a bf16 value exactly down to 2^-31 of it, and 2^-39 of it is the rounding
+  uint32_t qf[NT][4 * CH][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = tile * ROWS + n * 8 + r;
+    uint32_t (&w)[4 * CH][2] = qf[n];  // bf16 pairs first
+#pragma unroll
+    for (int i = 0; i < 8 * CH; ++i) w[i / 2][i % 2] = 0;
+    if (row < rows) {
+      const int token = by.group.div(row);
+      const uint4* p = reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.q + ((int64_t)seq * d.q_len + token) * d.ldq +
+                                                      (h * group + row - token * group) * DH);
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 v = p[k * 8 + c * 2 + i];
+          w[k * 4 + i * 2][0] = v.x, w[k * 4 + i * 2][1] = v.y, w[k * 4 + i * 2 + 1][0] = v.z, w[k * 4 + i * 2 + 1][1] = v.w;
+        }
+    }
+  }
+
   const PaSpan sp = page_attn_span(d, ctx, by.group.div(min(rows, (tile + 1) * ROWS) - 1));
   if (threadIdx.x == 0 && ctx > (int64_t)d.max_pages * d.page && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
   const int u_end = min(sp.units, (split + 1) * sp.per);
@@ -232,37 +256,13 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
     cp_commit();
   };
 
-  // query fragments: column r of each tile, the dims of this lane's key bytes, times
-  // a power of two that brings the tile's largest value to [2^14, 2^15): f16 then
-  // holds a bf16 value exactly down to 2^-31 of it, and 2^-39 of it is the rounding
-  uint32_t qf[NT][4 * CH][2];
-  int lim[NT][2];
-  float amax = 0.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int row = tile * ROWS + n * 8 + r;
-    uint32_t (&w)[4 * CH][2] = qf[n];  // bf16 pairs first
-#pragma unroll
-    for (int i = 0; i < 8 * CH; ++i) w[i / 2][i % 2] = 0;
-    if (row < rows) {
-      const int token = by.group.div(row);
-      const uint4* p = reinterpret_cast<const uint4*>((const __nv_bfloat16*)d.q + ((int64_t)seq * d.q_len + token) * d.ldq +
-                                                      (h * group + row - token * group) * DH);
-#pragma unroll
-      for (int k = 0; k < CH; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 v = p[k * 8 + c * 2 + i];
-          w[k * 4 + i * 2][0] = v.x, w[k * 4 + i * 2][1] = v.y, w[k * 4 + i * 2 + 1][0] = v.z, w[k * 4 + i * 2 + 1][1] = v.w;
-        }
-    }
-  }
-
   float2 scales[R::STAGES];  // of the units in flight, the next one first
 #pragma unroll
   for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, pg[s], scales[s]);
   int pg_next = pg[R::STAGES];
 
+  int lim[NT][2];
+  float amax = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
