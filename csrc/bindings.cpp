@@ -1261,7 +1261,7 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
   TORCH_CHECK(max_ctx < (1ll << 31) - 64, "page_attention: contexts of fewer than 2^31 tokens");
   lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)max_ctx, &d.nsplit, &d.min_units);
   torch::Tensor part;  // allocated per call: the allocator knows the stream
-  if (d.nsplit > 1) {
+  if (d.nsplit > 16) {
     const int64_t parts = q.size(0) * Hq * d.nsplit;
     part = torch::empty({parts * (Dh + 4)}, q.options().dtype(torch::kFloat32));
     d.part_ml = part.data_ptr<float>();

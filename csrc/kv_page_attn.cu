@@ -51,6 +51,7 @@ namespace lk {
 
 constexpr int PA_WARPS = 4;
 constexpr int PA_STAGES = 2;  // units on their way per warp (1 with 4 blocks an SM, 3 with 2: 7 to 15 % slower)
+constexpr int PA_CLUSTER = 16;     // parts that one cluster of blocks joins
 constexpr int PA_UNIT = 32;        // tokens a warp takes at a time (two M = 16 tiles)
 constexpr float PA_LOW = -3.0e38f;  // reference before the first token
 constexpr float PA_TOP = 14.f, PA_AIM = 7.f;
@@ -110,6 +111,17 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr));
+  return x;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr));
+  return x;
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -210,7 +222,8 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
   if (threadIdx.x == 0 && ctx > (int64_t)d.max_pages * d.page && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
   const int u_end = min(sp.units, (split + 1) * sp.per);
   cudaTriggerProgrammaticLaunchCompletion();  // the join may be brought up; it waits for all of this grid
-  if (split > 0 && split * sp.per >= sp.units) return;
+  const bool cluster = nsplit > 1 && nsplit <= PA_CLUSTER;  // the parts' blocks are a cluster and join by themselves
+  if (!cluster && split > 0 && split * sp.per >= sp.units) return;
   int u = split * sp.per + warp;
   if (nsplit > 1) {
 #pragma unroll
@@ -468,6 +481,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
       if (r == 0) *reinterpret_cast<float4*>(row + DH) = make_float4(ms[n][q], mw[n][q], x, 0.f);
     }
   __syncthreads();
+  float* joined = part + PA_WARPS * ROWS * PITCH;  // this block's rows, for the cluster
   for (int rl = warp; rl < ROWS; rl += PA_WARPS) {
     const int row = tile * ROWS + rl;
     if (row >= rows) break;
@@ -495,6 +509,11 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
       const float f = L == 0.f ? 0.f : fast_exp2(MW - MS) / L;
 #pragma unroll
       for (int i = 0; i < DH / 32; ++i) ((__nv_bfloat16*)d.out)[grow * d.ldo + head * DH + i * 32 + lane] = __float2bfloat16(o[i] * f);
+    } else if (cluster) {
+      float* y = joined + rl * PITCH;
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) y[i * 32 + lane] = o[i];
+      if (lane == 0) *reinterpret_cast<float4*>(y + DH) = make_float4(MS, MW, L, 0.f);
     } else {
       const int64_t at = (grow * d.Hq + head) * nsplit + split;
 #pragma unroll
@@ -502,6 +521,34 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
       if (lane == 0) *reinterpret_cast<float4*>(d.part_ml + at * 4) = make_float4(MS, MW, L, 0.f);
     }
   }
+  if (!cluster) return;
+  // the cluster's blocks share the rows out and read each other's parts, in their order
+  cluster_sync();
+  for (int rl = split + nsplit * warp; rl < ROWS; rl += nsplit * PA_WARPS) {
+    const int row = tile * ROWS + rl;
+    if (row >= rows) break;
+    const uint32_t mine = smem_u32(joined + rl * PITCH);
+    float4 ml = make_float4(PA_LOW, PA_LOW, 0.f, 0.f);
+    if (lane < nsplit) ml = ld_cluster4(mapa_shared(mine + DH * 4, lane));
+    const float MS = warp_max(ml.x), MW = warp_max(ml.y);
+    const float L = warp_sum(ml.z * fast_exp2(ml.x - MS)), f = fast_exp2(ml.y - MW);
+    float o[DH / 32];
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int q = 0; q < nsplit; ++q) {
+      const float g = __shfl_sync(0xffffffffu, f, q);
+      const uint32_t there = mapa_shared(mine + lane * 4, q);
+#pragma unroll
+      for (int i = 0; i < DH / 32; ++i) o[i] = fmaf(ld_cluster(there + i * 128), g, o[i]);
+    }
+    const int token = by.group.div(row), head = h * group + row - token * group;
+    const float g = L == 0.f ? 0.f : fast_exp2(MW - MS) / L;
+#pragma unroll
+    for (int i = 0; i < DH / 32; ++i)
+      ((__nv_bfloat16*)d.out)[((int64_t)seq * d.q_len + token) * d.ldo + head * DH + i * 32 + lane] = __float2bfloat16(o[i] * g);
+  }
+  cluster_sync();  // no block leaves while another reads its shared memory
 }
 
 // Joins the parts of a (row, head), a block each: every warp finds the references and
@@ -571,33 +618,45 @@ static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
   const int64_t blocks = (int64_t)d.num_seqs * d.Hkv * tiles * d.nsplit;
   LK_REQUIRE(blocks < (1ll << 31) && (int64_t)d.num_seqs * d.q_len * d.Hq < (1ll << 31),
              "page_attention: too many rows in one call");
-  constexpr int merge = PA_WARPS * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
+  constexpr int merge = (PA_WARPS + 1) * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
   constexpr int smem = ring > merge ? ring : merge;
   auto k = page_attn_kernel<KV, DH, NT>;
-  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
+  static std::atomic<uint64_t> ready{0};  // devices whose kernel attributes are set
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return check_launch("page_attention: shared memory");
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return check_launch("page_attention: kernel attributes");
     ready.fetch_or(bit);
   }
-  k<<<(unsigned)blocks, 32 * PA_WARPS, smem, s>>>(
-      d, PaDivs{FastDiv(d.nsplit), FastDiv(d.Hkv), FastDiv(tiles), FastDiv(d.Hq / d.Hkv), FastDiv(d.page)});
+  const bool cluster = d.nsplit > 1 && d.nsplit <= PA_CLUSTER;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(32 * PA_WARPS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  cfg.attrs = &attr;
+  if (cluster) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = d.nsplit;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  cudaLaunchKernelEx(&cfg, k, d, PaDivs{FastDiv(d.nsplit), FastDiv(d.Hkv), FastDiv(tiles), FastDiv(d.Hq / d.Hkv), FastDiv(d.page)});
   if (check_launch("page_attention")) return -1;
-  if (d.nsplit == 1) return 0;
+  if (d.nsplit == 1 || cluster) return 0;
   const int64_t joins = (int64_t)d.num_seqs * d.q_len * d.Hq;
   // launched while the parts still run (its blocks wait for them in the launch order of
   // the stream): the launch's own latency is not waited for
-  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)joins);
   cfg.blockDim = dim3(32 * JOIN_WARPS);
-  cfg.stream = s;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
+  cfg.dynamicSmemBytes = 0;
+  attr = cudaLaunchAttribute{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, page_attn_join_kernel<DH>, d, 8 * NT, d.nsplit);
   return check_launch("page_attention_join");
@@ -614,7 +673,7 @@ using namespace lk;
 //   an SM), times the parts of an SM - half of the time the fullest SM decides (equal
 //   lengths), half the mean, of lengths that are 0.6 of the longest;
 //   but no less than the longest part alone, at the 60 % of the rate that one block reaches;
-//   300 more for a second launch.
+//   60 more for the join of a cluster, 300 for a second launch.
 // Measured (us; uncut, chosen, best): 2 contexts of 100003: 731, 64 (18 parts), 64; 8
 // sequences of up to 4096 (8 KV heads of 128): 39, 19, 17; 32: 46, 40, 40; 256: 186, uncut.
 // Beyond what fills the GPU only contexts over 4096 are cut, so that one does not run on
@@ -628,11 +687,13 @@ extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hk
   auto consider = [&](int64_t ns) {
     if (ns < 1 || ns > full) return;
     const double part = (double)max_ctx / ns + 150, mean = 0.6 * blocks * ns / sms;
-    const double cost = std::max(part * 0.5 * ((double)((blocks * ns + sms - 1) / sms) + mean), part / 0.6) + (ns > 1 ? 300 : 0);
+    const double cost = std::max(part * 0.5 * ((double)((blocks * ns + sms - 1) / sms) + mean), part / 0.6) +
+                        (ns > PA_CLUSTER ? 300 : ns > 1 ? 60 : 0);
     if (cost < least) least = cost, best = (int)ns;
   };
   for (int ns = 1; ns <= full; ns += step) consider(ns);
   for (int k = 1; k <= 3; ++k) consider((int64_t)k * sms / blocks);
+  consider(PA_CLUSTER);
   *nsplit = best > 1 ? best : std::max(1, cdiv(max_ctx, 4096));
   *min_units = best > 1 ? 256 / PA_UNIT : 4096 / PA_UNIT;
 }
@@ -640,7 +701,7 @@ extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hk
 extern "C" int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s) {
   LK_REQUIRE(d->Dh == 64 || d->Dh == 128, "page_attention: head_dim must be 64 or 128");
   if (d->num_seqs == 0) return 0;
-  LK_REQUIRE(d->nsplit == 1 || (d->part_o && d->part_ml), "page_attention: split partial buffers needed");
+  LK_REQUIRE(d->nsplit <= PA_CLUSTER || (d->part_o && d->part_ml), "page_attention: split partial buffers needed");
   const bool wide = d->Hq / d->Hkv * d->q_len > 8;
 #define LK_PA(KV, DH) return wide ? launch_page_attn<KV, DH, 2>(*d, s) : launch_page_attn<KV, DH, 1>(*d, s)
   if (d->kv_dtype == 1) {

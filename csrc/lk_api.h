@@ -493,7 +493,7 @@ typedef struct LkPageAttnDesc {
   void* out;  // [num_seqs * q_len, Hq*Dh] bf16
   int64_t ldo;
   int nsplit, min_units;  // parts of each context (lk_page_attention_splits)
-  float* part_o;   // [num_seqs * q_len, Hq, nsplit, Dh] when nsplit > 1
+  float* part_o;   // [num_seqs * q_len, Hq, nsplit, Dh] when nsplit > 16 (fewer parts join in their cluster)
   float* part_ml;  // [num_seqs * q_len, Hq, nsplit, 4]
   int kv_dtype;
   int* status;
