@@ -3,6 +3,7 @@
 // the launcher on the current CUDA stream; launcher errors become Python
 // RuntimeErrors.  No binding falls back to another implementation.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -1168,6 +1169,11 @@ int page_cache(const char* op, const torch::Tensor& k, const torch::Tensor& v, c
   return dt == torch::kFloat8_e4m3fn ? 1 : 2;
 }
 
+// An uninitialised tensor beside `like`, without the dispatcher (about 0.5 us less a call).
+torch::Tensor empty_beside(const torch::Tensor& like, at::IntArrayRef size, c10::ScalarType dt) {
+  return at::detail::empty_cuda(size, dt, like.device(), c10::nullopt);
+}
+
 void same_device(const char* op, const torch::Tensor& a, std::initializer_list<const torch::Tensor*> others) {
   for (const torch::Tensor* t : others)
     TORCH_CHECK(t->device() == a.device(), op, ": tensors are on ", a.device().str(), " and ", t->device().str());
@@ -1203,7 +1209,7 @@ torch::Tensor page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::T
   const c10::cuda::CUDAGuard g(k_cache.device());
   need_contig(slots, "slots", torch::kInt32);
   torch::Tensor out = out_opt.has_value() ? *out_opt
-                                          : torch::empty({slots.numel(), 2 * Hkv * Dh}, k_scale.options().dtype(torch::kBFloat16));
+                                          : empty_beside(k_cache, {slots.numel(), 2 * Hkv * Dh}, torch::kBFloat16);
   need(out, "out", torch::kBFloat16);
   TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == slots.numel() && out.size(1) == 2 * Hkv * Dh,
               "page_gather: out must be row-major [n, 2 * Hkv * Dh]");
@@ -1241,7 +1247,7 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
               "page_attention: one table row and one length per sequence");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && (q.stride(0) % 8 == 0 || q.size(0) <= 1),
               "page_attention: the rows of q must be 16-byte aligned");
-  torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({q.size(0), Hq * Dh}, q.options());
+  torch::Tensor out = out_opt.has_value() ? *out_opt : empty_beside(q, {q.size(0), Hq * Dh}, torch::kBFloat16);
   need(out, "out", torch::kBFloat16);
   TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == q.size(0) && out.size(1) == Hq * Dh,
               "page_attention: out must be row-major [sequences * q_len, Hq * Dh]");
@@ -1263,7 +1269,7 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
   torch::Tensor part;  // allocated per call: the allocator knows the stream
   if (d.nsplit > 16) {
     const int64_t parts = q.size(0) * Hq * d.nsplit;
-    part = torch::empty({parts * (Dh + 4)}, q.options().dtype(torch::kFloat32));
+    part = empty_beside(q, {parts * (Dh + 4)}, torch::kFloat32);
     d.part_ml = part.data_ptr<float>();
     d.part_o = d.part_ml + parts * 4;
   }
@@ -1312,7 +1318,7 @@ torch::Tensor adjust_logits(torch::Tensor logits, c10::optional<torch::Tensor> c
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
               "adjust_logits: logits must be a row-major CUDA tensor [n, vocab]");
   const int64_t n = logits.size(0), vocab = logits.size(1);
-  torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({n, vocab}, logits.options());
+  torch::Tensor out = out_opt.has_value() ? *out_opt : empty_beside(logits, {n, vocab}, logits.scalar_type());
   need(out, "out", logits.scalar_type());
   TORCH_CHECK(out.dim() == 2 && out.stride(1) == 1 && out.size(0) == n && out.size(1) == vocab,
               "adjust_logits: out must be row-major [n, vocab]");
