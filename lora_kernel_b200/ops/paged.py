@@ -54,7 +54,8 @@ def page_attention(q: torch.Tensor, k_cache, v_cache, k_scale, v_scale, block_ta
 
     block_tables int32 [n, pages], ctx_lens int32 [n] (the q_len tokens
     included; 0 = unused row, which gives zeros).  Query j attends to positions
-    0 .. ctx - q_len + j.  max_ctx: the longest length, where the host knows
+    0 .. ctx - q_len + j; the codes there are page_append's, which are finite
+    (what lies in a page beyond a context is never read).  max_ctx: the longest length, where the host knows
     it (0: the tables' width); it only guides how the work is split."""
     require_device(q)
     return C().page_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, page, Hq, Hkv, Dh, q_len,

@@ -229,7 +229,10 @@ class ModelRunner:
             bits = np.zeros((len(which), (V + 31) // 32 * 32), dtype=np.uint8)
             at = [-1] * len(allowed)
             for m, k in enumerate(which):
-                bits[m, np.asarray(allowed[k], dtype=np.int64)] = 1
+                ids = np.asarray(allowed[k], dtype=np.int64)
+                if ids.size and not 0 <= ids.min() <= ids.max() < V:
+                    raise ValueError(f"a grammar allows token ids outside [0, {V})")
+                bits[m, ids] = 1
                 at[k] = m
             words = np.packbits(bits, axis=1, bitorder="little").view(np.int32)
             mask = torch.from_numpy(words).to(dev)

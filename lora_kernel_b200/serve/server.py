@@ -272,6 +272,7 @@ def create_app(engine: LLMEngine, model_name: str = "lora-kernel-b200", api_keys
     keys = set(api_keys)
     adjust = all(getattr(getattr(e, "runner", None), "supports_adjust", False) for e in engines)
     validator = validator or InputValidator(engine.cfg.vocab_size, adjust=adjust)
+    adjust = adjust and getattr(validator, "adjust", False)  # a validator that does not check these fields: they are not read
     masker = PIIMasker() if pii_filter else None
     signer = RequestSigner(signing_secret) if signing_secret else None
 

@@ -229,6 +229,23 @@ def test_attention_long(kind, Hq, Hkv, Dh, q_len, ctxs):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("Hq,Hkv,Dh,q_len,ctxs", [
+    (8, 1, 128, 1, [3900]), (6, 1, 128, 3, [4100]), (2, 1, 64, 1, [5003]), (16, 2, 64, 2, [4000, 10, 0, 2500]), (12, 2, 128, 1, [1025, 1024]),
+    (24, 2, 64, 5, [3000, 777])])
+def test_attention_parts(kind, Hq, Hkv, Dh, q_len, ctxs):
+    """Contexts cut into 2 to 16 parts, joined by their cluster, and (a longer bound) into more, joined by a second
+    launch: both against the oracle; parts without a token among them."""
+    (k, v, ks, vs), bt, refs = _filled(kind, ctxs, 16, Hkv, Dh, 81)
+    q = torch.randn(len(ctxs) * q_len, Hq * Dh, device=dev, generator=torch.Generator(device=dev).manual_seed(1)).to(torch.bfloat16)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=dev)
+    wide = torch.cat([bt, torch.full((len(ctxs), 8000), -1, dtype=torch.int32, device=dev)], dim=1)
+    for table, max_ctx in ((bt, max(ctxs)), (bt, 0), (wide, 0), (wide, 1000)):
+        out = P().page_attention(q, k, v, ks, vs, table, ctx, 16, Hq, Hkv, Dh, q_len=q_len, max_ctx=max_ctx)
+        _check_attention(out, q, refs, ctxs, q_len, Hq, Dh)
+    assert _status_code() == ""
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_scales_far_apart(kind):
     """Pages whose values differ by 2^40: a query that looks at a page of small values still sees them."""
     Hq, Hkv, Dh, page, ctxs = 4, 1, 64, 8, [200, 31]
