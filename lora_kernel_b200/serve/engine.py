@@ -116,6 +116,9 @@ class Request:
     on_token: Optional[Callable[["Request", int], None]] = None
     samples: List[int] = field(default_factory=list)  # ids of the other samples (params.n > 1)
     counts_row: int = -1        # row of the runner's token counts
+    # params.allowed_token_ids (without a grammar) and logit_bias as the runner packs them, once
+    fixed_mask: Optional[object] = None
+    fixed_bias: Optional[object] = None
 
     @property
     def tokens(self) -> List[int]:
@@ -389,7 +392,23 @@ class LLMEngine:
         return self.runner.adjust_logits(
             logits, [r.counts_row if r.params.penalised else -1 for r in reqs],
             [(p.repetition_penalty, p.frequency_penalty, p.presence_penalty) for p in ps],
-            [p.logit_bias for p in ps], allowed)
+            [self._packed_bias(r) for r in reqs], [self._packed_mask(r, a) for r, a in zip(reqs, allowed)])
+
+    def _packed_mask(self, r: Request, allowed):
+        pack = getattr(self.runner, "pack_allowed", None)
+        if allowed is None or pack is None or r.params.grammar is not None:
+            return allowed
+        if r.fixed_mask is None:
+            r.fixed_mask = pack(allowed)
+        return r.fixed_mask
+
+    def _packed_bias(self, r: Request):
+        pack = getattr(self.runner, "pack_bias", None)
+        if not r.params.logit_bias or pack is None:
+            return r.params.logit_bias
+        if r.fixed_bias is None:
+            r.fixed_bias = pack(r.params.logit_bias)
+        return r.fixed_bias
 
     def _sample(self, reqs: List[Request], logits: torch.Tensor) -> List[Optional[int]]:
         allowed = [r.params.allowed(r.output) if r.params.adjusts else None for r in reqs]

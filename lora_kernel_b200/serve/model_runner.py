@@ -31,7 +31,7 @@ import math
 from dataclasses import dataclass
 
 import numpy as np
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -214,31 +214,48 @@ class ModelRunner:
         """Count the sampled tokens [n] (row -1: a request without penalties)."""
         LG.add_token_counts(self._counts, torch.tensor(rows, dtype=torch.int32, device=self.device), tokens)
 
+    def pack_allowed(self, ids: Sequence[int]) -> np.ndarray:
+        """A set of allowed token ids as mask words (int32 [ceil(vocab / 32)], a bit per token)."""
+        V = self.cfg.vocab_size
+        ids = np.asarray(ids, dtype=np.int64)
+        if ids.size and not 0 <= ids.min() <= ids.max() < V:
+            raise ValueError(f"allowed token ids outside [0, {V})")
+        bits = np.zeros((V + 31) // 32 * 32, dtype=np.uint8)
+        bits[ids] = 1
+        return np.packbits(bits, bitorder="little").view(np.int32)
+
+    @staticmethod
+    def pack_bias(bias: Dict[int, float]) -> Tuple[np.ndarray, np.ndarray]:
+        """{token id: bias} as (ids int32, values fp32)."""
+        return np.fromiter(bias.keys(), np.int32, len(bias)), np.fromiter(bias.values(), np.float32, len(bias))
+
     def adjust_logits(self, logits: torch.Tensor, rows: List[int], penalties: List[Tuple[float, float, float]],
-                      biases: List[Optional[Dict[int, float]]], allowed: List[Optional[List[int]]]) -> torch.Tensor:
+                      biases: List, allowed: List) -> torch.Tensor:
         """logits [n, vocab] changed in place: each request's penalties (row of the
-        counts table, -1 = none), biases {token: bias} and, where given, the only
-        tokens that its grammar allows."""
-        dev, V = self.device, self.cfg.vocab_size
-        counts = rows_t = pen = mask = mask_rows = None
-        if any(r >= 0 for r in rows):
-            counts, rows_t = self._counts, torch.tensor(rows, dtype=torch.int32, device=dev)
-            pen = torch.tensor(penalties, dtype=torch.float32, device=dev)
+        counts table, -1 = none), biases ({token: bias}, or its pack_bias arrays) and,
+        where given, the only tokens that its grammar allows (token ids, or their
+        pack_allowed words)."""
+        n, V = len(rows), self.cfg.vocab_size
         which = [k for k, a in enumerate(allowed) if a is not None]
+        mask = None
+        at = np.full(n, -1, dtype=np.int32)
         if which:
-            bits = np.zeros((len(which), (V + 31) // 32 * 32), dtype=np.uint8)
-            at = [-1] * len(allowed)
-            for m, k in enumerate(which):
-                ids = np.asarray(allowed[k], dtype=np.int64)
-                if ids.size and not 0 <= ids.min() <= ids.max() < V:
-                    raise ValueError(f"a grammar allows token ids outside [0, {V})")
-                bits[m, ids] = 1
-                at[k] = m
-            words = np.packbits(bits, axis=1, bitorder="little").view(np.int32)
-            mask = torch.from_numpy(words).to(dev)
-            mask_rows = torch.tensor(at, dtype=torch.int32, device=dev)
-        return LG.adjust_logits(logits, counts, rows_t, pen, bias=LG.logit_bias(biases, dev), mask=mask,
-                                mask_rows=mask_rows, out=logits)
+            at[which] = np.arange(len(which), dtype=np.int32)
+            mask = torch.from_numpy(np.stack([a if isinstance(a, np.ndarray) else self.pack_allowed(a)
+                                              for a in allowed if a is not None])).to(self.device)
+        # the small arrays travel as one upload of 32-bit words
+        none = (np.zeros(0, dtype=np.int32), np.zeros(0, dtype=np.float32))
+        biases = [b if isinstance(b, tuple) else self.pack_bias(b) if b else none for b in biases]
+        offsets = np.zeros(n + 1, dtype=np.int32)
+        np.cumsum([len(b[0]) for b in biases], out=offsets[1:])
+        parts = [np.asarray(rows, dtype=np.int32), at, np.asarray(penalties, dtype=np.float32).reshape(-1).view(np.int32), offsets,
+                 np.concatenate([b[0] for b in biases]), np.concatenate([b[1] for b in biases]).view(np.int32)]
+        rows_t, at_t, pen, off, ids, values = torch.from_numpy(np.concatenate(parts)).to(self.device).split([len(p) for p in parts])
+        counted = any(r >= 0 for r in rows)
+        return LG.adjust_logits(logits, self._counts if counted else None, rows_t if counted else None,
+                                pen.view(torch.float32).view(n, 3) if counted else None,
+                                bias=(off, ids, values.view(torch.float32)) if len(ids) else None, mask=mask,
+                                mask_rows=at_t if which else None, out=logits)
 
     def sample(self, logits: torch.Tensor, temps: Optional[List[float]], seed: int,
                top_ps: Optional[List[float]] = None, row_seeds: Optional[List[int]] = None) -> torch.Tensor:
