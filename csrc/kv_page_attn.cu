@@ -75,10 +75,11 @@ struct PaRing {
     if constexpr (DH == 128) return t * 128 + ((k ^ (t & 6) ^ ((t & 1) << 2)) << 4);
     else return (t >> 1) * 128 + ((((t & 1) << 2 | k) ^ (t & 6)) << 4);
   }
-  // the token of the unit that a lane copies a chunk of with its copy i
+  // the token of the unit that a lane copies a chunk of with its copy i, and where to: i * 512
+  // and what the lane and the parity of i say (at head_dim 64 the lane alone)
   static constexpr int LANES = DH / 16;  // lanes per row
   static __device__ __forceinline__ int token(int i, int lane) { return i * (32 / LANES) + lane / LANES; }
-  static __device__ __forceinline__ uint32_t place(int i, int lane) { return at(token(i, lane), lane % LANES); }
+  static __device__ __forceinline__ uint32_t place(int odd, int lane) { return at(token(odd, lane), lane % LANES) - odd * 512; }
 };
 
 // 16 bytes to shared address dst + OFF (a constant that stays in the instruction);
@@ -98,6 +99,13 @@ __device__ __forceinline__ void static_for_each(F f, std::integer_sequence<int, 
 template <int N, typename F>  // f(0), ..., f(N - 1), each argument a constant
 __device__ __forceinline__ void static_for(F f) {
   static_for_each(f, std::make_integer_sequence<int, N>{});
+}
+// p + n * stride bytes in one multiply-add
+template <typename T>
+__device__ __forceinline__ const T* advance(const T* p, uint32_t n, uint32_t stride) {
+  const T* q;
+  asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(q) : "r"(n), "r"(stride), "l"(p));
+  return q;
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -183,13 +191,16 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int ctx = d.ctx_lens[seq];
   const int* table = d.tables + (int64_t)seq * d.max_pages;
+  struct Place {
+    int page, row;  // page id and row in the page
+  };
   auto page_of = [&](int u) {  // of this lane's token of unit u; anything beyond the context is not used
-    const int i = by.page.div(u * PA_UNIT + lane);
-    return i < d.max_pages ? table[i] : 0;
+    const int t = u * PA_UNIT + lane, i = by.page.div(t);
+    return Place{i < d.max_pages ? table[i] : 0, t - i * d.page};
   };
   // an uncut context begins at unit `warp` whatever its length: its pages are looked up
   // while the length is on its way
-  int pg[PA_STAGES + 1];
+  Place pg[PA_STAGES + 1];
   if (nsplit == 1) {
 #pragma unroll
     for (int s = 0; s <= PA_STAGES; ++s) pg[s] = page_of(warp + s * PA_WARPS);
@@ -240,29 +251,29 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
   // the unit's copies: this lane looks up token `lane`, then copies 16 bytes of its share
   // of the rows (8 lanes a 128-byte line, so that a request is a whole line); its token's
   // scales go to registers and into the stage when the unit's turn comes
-  auto issue = [&](int u, int stage, int pg, float2& scales) {
+  const float* ks = d.k_scale + h;
+  const float* vs = d.v_scale + h;
+  const uint32_t to[2] = {ring_u + R::place(0, lane), ring_u + R::place(1, lane)};
+  auto issue = [&](int u, int stage, Place at, float2& scales) {
     if (u < u_end) {
-      const int t = u * PA_UNIT + lane;
-      const bool there = t < sp.end, ok = there && (unsigned)pg < (unsigned)d.num_pages;
+      const bool there = u * PA_UNIT + lane < sp.end, ok = there && (unsigned)at.page < (unsigned)d.num_pages;
       const unsigned valid = __ballot_sync(0xffffffffu, ok);
-      const uint32_t st = ring_u + stage * R::STAGE;
-      const uint32_t slot = ok ? pg * d.page + (t - by.page.div(t) * d.page) : 0;
-      const int64_t sc = ok ? (int64_t)pg * d.Hkv + h : 0;
-      scales = make_float2(d.k_scale[sc], d.v_scale[sc]);
-      if (lane == 0) asm volatile("st.shared.u32 [%0+%1], %2;" ::"r"(st), "n"(R::MASK), "r"(valid) : "memory");
+      const uint32_t page = ok ? at.page : 0, slot = ok ? page * d.page + at.row : 0, st = stage * R::STAGE;
+      scales = make_float2(*advance(ks, page, d.Hkv * 4), *advance(vs, page, d.Hkv * 4));
+      if (lane == 0) asm volatile("st.shared.u32 [%0+%1], %2;" ::"r"(ring_u + st), "n"(R::MASK), "r"(valid) : "memory");
       if (valid == 0xffffffffu) {
         static_for<DH / 16>([&](auto i) {
-          const uint64_t off = (uint64_t)__shfl_sync(0xffffffffu, slot, R::token(i, lane)) * tok_stride;
-          cp_async16<0>(st + R::place(i, lane), kbase + off);
-          cp_async16<R::KV_BYTES>(st + R::place(i, lane), vbase + off);
+          const uint32_t s = __shfl_sync(0xffffffffu, slot, R::token(i, lane));
+          cp_async16<i * 512>(to[i & 1] + st, advance(kbase, s, tok_stride));
+          cp_async16<i * 512 + R::KV_BYTES>(to[i & 1] + st, advance(vbase, s, tok_stride));
         });
       } else {  // the end of the context, or a bad page id: nothing is read there, zeros take its place
         if (there && !ok && d.status) atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
         static_for<DH / 16>([&](auto i) {
-          const uint64_t off = (uint64_t)__shfl_sync(0xffffffffu, slot, R::token(i, lane)) * tok_stride;
+          const uint32_t s = __shfl_sync(0xffffffffu, slot, R::token(i, lane));
           const bool on = (valid >> R::token(i, lane)) & 1;
-          cp_async16_or_zero<0>(st + R::place(i, lane), kbase + off, on);
-          cp_async16_or_zero<R::KV_BYTES>(st + R::place(i, lane), vbase + off, on);
+          cp_async16_or_zero<i * 512>(to[i & 1] + st, advance(kbase, s, tok_stride), on);
+          cp_async16_or_zero<i * 512 + R::KV_BYTES>(to[i & 1] + st, advance(vbase, s, tok_stride), on);
         });
       }
     }
@@ -272,7 +283,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
   float2 scales[R::STAGES];  // of the units in flight, the next one first
 #pragma unroll
   for (int s = 0; s < R::STAGES; ++s) issue(u + s * PA_WARPS, s, pg[s], scales[s]);
-  int pg_next = pg[R::STAGES];
+  Place pg_next = pg[R::STAGES];
 
   int lim[NT][2];
   float amax = 0.f;
