@@ -33,12 +33,12 @@
 // ones whichever the query looks at.  The softmax sum is kept in fp32 apart.
 //
 // Measured: 256 sequences of up to 4096 tokens (32 / 8 heads of 128, e4m3, 1084 MB)
-// 185-197 us, 84-89 % of the HBM copy rate; two of 100003 tokens 64-66 us (77-79 %,
-// join included); int8 codes take two instructions more a pair: 200 us.  A block costs
-// 3.5 us beside its tokens (length and pages, first data, merge), which is what the full
-// batch lacks, and at head_dim 64 more (67 us for a floor of 42).  Where rows are few, a
-// warp's 620 instructions per 32 tokens and their dependences bound it: 24 sequences of
-// up to 2047 tokens with five queries each (40 rows, 8 / 1 heads of 64) 23 us.
+// 182-193 us, 86-91 % of the HBM copy rate; two of 100003 tokens 64 us (79 %); int8 codes
+// take two instructions more a pair: 200 us.  A block costs 3.5 us beside its tokens
+// (launch, length and pages, first data, merge), which is what the full batch lacks, and
+// at head_dim 64 more (65 us for a floor of 42).  Where rows are few, a warp's 450
+// instructions per 32 tokens and their dependences bound it: 24 sequences of up to 2047
+// tokens with five queries each (40 rows, 8 / 1 heads of 64, int8) 22.5 us.
 #include <algorithm>
 #include <utility>
 
