@@ -36,7 +36,7 @@
 // 182-193 us, 86-91 % of the HBM copy rate; two of 100003 tokens 64 us (79 %); int8 codes
 // take two instructions more a pair: 200 us.  A block costs 3.5 us beside its tokens
 // (launch, length and pages, first data, merge), which is what the full batch lacks, and
-// at head_dim 64 more (65 us for a floor of 42).  Where rows are few, a warp's 450
+// at head_dim 64 more (65 us for a floor of 42).  Where rows are few, a warp's 480
 // instructions per 32 tokens and their dependences bound it: 24 sequences of up to 2047
 // tokens with five queries each (40 rows, 8 / 1 heads of 64, int8) 22.5 us.
 #include <algorithm>

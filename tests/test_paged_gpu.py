@@ -384,6 +384,33 @@ def test_attention_streams_and_graphs():
         _check_attention(out, q, [(a[:c], b[:c]) for (a, b), c in zip(refs, lens)], lens, 1, Hq, Dh)
 
 
+def test_long_context_in_a_graph():
+    """More parts than a cluster joins (a second launch that starts early), captured and replayed over changing lengths,
+    with another kernel's output as its query."""
+    Hq, Hkv, Dh, page, c = 4, 1, 64, 16, 20000
+    (k, v, ks, vs), bt, refs = _filled("fp8_page", [c], page, Hkv, Dh, 65)
+    q0 = torch.randn(1, Hq * Dh, device=dev, generator=torch.Generator(device=dev).manual_seed(2)).to(torch.bfloat16)
+    ctx = torch.tensor([c], dtype=torch.int32, device=dev)
+
+    def call():
+        q = q0 * 2
+        out = P().page_attention(q, k, v, ks, vs, bt, ctx, page, Hq, Hkv, Dh, max_ctx=c)
+        return out + 1  # reads the result at once
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for n in (c, 1, 0, 333, c - 1):
+        ctx.fill_(n)
+        graph.replay()
+        graph.replay()
+        want, mag = O.attention((q0 * 2).double().view(1, Hq, Dh), *[x[:n] for x in refs[0]], n, 1)
+        err = (out.double().view(1, Hq, Dh) - 1 - want).abs()
+        assert (err <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * mag + 2.0 ** -8).all()  # + 1 in bf16: 2^-8
+
+
 def test_attention_repeats_to_the_bit():
     Hq, Hkv, Dh, page, ctxs = 4, 1, 128, 16, [9000, 333]
     (k, v, ks, vs), bt, _ = _filled("fp8_page", ctxs, page, Hkv, Dh, 71)
