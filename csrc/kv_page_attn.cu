@@ -685,8 +685,9 @@ using namespace lk;
 //   lengths), half the mean, of lengths that are 0.6 of the longest;
 //   but no less than the longest part alone, at the 60 % of the rate that one block reaches;
 //   60 more for the join of a cluster, 300 for a second launch.
-// Measured (us; uncut, chosen, best): 2 contexts of 100003: 731, 64 (18 parts), 64; 8
-// sequences of up to 4096 (8 KV heads of 128): 39, 19, 17; 32: 46, 40, 40; 256: 186, uncut.
+// Measured (us on the device; uncut, chosen, best of 1 to 16 parts): one sequence of 2000
+// tokens 16.3, 6.7, 6.7; 8 of up to 4096 35, 13.8, 13.7; 32 of them 42, 35, 35; 64 of them 62,
+// 62, 59; 256 uncut 182. More than 16 parts: one of 30000 19.6 (16 parts 23.6), two of 100003 64.
 // Beyond what fills the GPU only contexts over 4096 are cut, so that one does not run on
 // alone.
 extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units) {

@@ -284,9 +284,10 @@ extern "C" int lk_adjust_logits(const LkAdjustLogitsDesc* d, cudaStream_t s) {
   const int each = d->f32 ? 4 : 2;
   const bool vec = rows_aligned(d->logits, d->ld, each, d->n) && rows_aligned(d->out, d->ldo, each, d->n) &&
                    (!d->counts || rows_aligned(d->counts, d->ldc, 2, d->count_rows));
-  // long spans share the search for a row's biases and have more loads on their way; short
-  // ones fill the GPU
-  const int groups = (int64_t)d->n * cdiv(d->vocab, ADJ_GROUPS * ADJ_STEP) >= 4 * num_sms() ? ADJ_GROUPS : 1;
+  // two groups a thread share the search for a row's biases and have more loads on their way,
+  // one fills the GPU sooner (us with 1 / 2 groups, 300 biases a row, 128256 columns: 1 row 2.6 /
+  // 3.1, 8 rows 3.6 / 3.4, 16 rows 4.9 / 4.4, 64 rows 12.1 / 9.8)
+  const int groups = (int64_t)d->n * cdiv(d->vocab, ADJ_GROUPS * ADJ_STEP) >= 2 * num_sms() ? ADJ_GROUPS : 1;
   const dim3 grid(cdiv(d->vocab, groups * ADJ_STEP), d->n);
   const int smem = d->bias_offsets ? groups * (ADJ_STEP + ADJ_STEP / 32) * 4 : 0;
 #define LK_ADJ(T, VEC)                                                                           \

@@ -274,9 +274,10 @@ class ModelRunner:
             return SV.sample_topp(logits, t, p, seed, row_seeds=rs)
         return SV.sample(logits, t, seed)
 
-    # a chunk of up to this many rows attends to the pages themselves instead of a bf16 copy
-    # of its context
-    PAGE_ATTN_ROWS = 16
+    # A chunk of up to this many rows attends to the pages themselves instead of a bf16 copy
+    # of its context (us, 32 / 8 heads of 128, pages / copy and flash kernel: 16 rows over 2000
+    # tokens 10 / 37, over 8000 31 / 126; 64 rows 30 / 38 and 70 / 126; 128 rows 36 / 40, 97 / 128)
+    PAGE_ATTN_ROWS = 128
 
     # -------------------------------------------------------------- prefill
     @torch.no_grad()
