@@ -40,6 +40,7 @@
 // instructions per 32 tokens and their dependences bound it: 24 sequences of up to 2047
 // tokens with five queries each (40 rows, 8 / 1 heads of 64, int8) 22.5 us.
 #include <algorithm>
+#include <mutex>
 #include <utility>
 
 #include "common.cuh"
@@ -624,53 +625,91 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) page_attn_join_kernel(LkPageA
 }
 
 template <int KV, int DH, int NT>
-static int launch_page_attn(const LkPageAttnDesc& d, cudaStream_t s) {
-  const int rows = d.Hq / d.Hkv * d.q_len, tiles = cdiv(rows, 8 * NT);
-  const int64_t blocks = (int64_t)d.num_seqs * d.Hkv * tiles * d.nsplit;
-  LK_REQUIRE(blocks < (1ll << 31) && (int64_t)d.num_seqs * d.q_len * d.Hq < (1ll << 31),
-             "page_attention: too many rows in one call");
-  constexpr int merge = (PA_WARPS + 1) * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
-  constexpr int smem = ring > merge ? ring : merge;
-  auto k = page_attn_kernel<KV, DH, NT>;
-  static std::atomic<uint64_t> ready{0};  // devices whose kernel attributes are set
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-        cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return check_launch("page_attention: kernel attributes");
-    ready.fetch_or(bit);
+struct PaKernel {
+  static constexpr int merge = (PA_WARPS + 1) * 8 * NT * (DH + 4) * 4, ring = PA_WARPS * PaRing<DH>::WARP;
+  static constexpr int smem = ring > merge ? ring : merge;
+
+  static void config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, int64_t blocks, int nsplit) {
+    cfg = cudaLaunchConfig_t{};
+    attr = cudaLaunchAttribute{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(32 * PA_WARPS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    if (nsplit > 1 && nsplit <= PA_CLUSTER) {
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = nsplit;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.numAttrs = 1;
+    }
   }
-  const bool cluster = d.nsplit > 1 && d.nsplit <= PA_CLUSTER;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(32 * PA_WARPS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  cfg.attrs = &attr;
-  if (cluster) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = d.nsplit;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+
+  // Kernel attributes of the current device, set once; and how many blocks it holds at a time
+  // when they come in clusters of c (0: singly), which the GPU's partition limits: of 2
+  // blocks an SM on 148 SMs 296 singly, 270 by sixes, 224 by sixteens.
+  static const int* places() {
+    struct Table {
+      std::once_flag once;
+      int at[PA_CLUSTER + 1] = {0};
+    };
+    static Table tables[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    Table& t = tables[dev & 63];
+    std::call_once(t.once, [&] {
+      auto k = page_attn_kernel<KV, DH, NT>;
+      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+          cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return;
+      int blocks = 0;
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k, 32 * PA_WARPS, smem) != cudaSuccess) return;
+      t.at[0] = t.at[1] = blocks * num_sms();
+      for (int c = 2; c <= PA_CLUSTER; ++c) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr;
+        config(cfg, attr, (int64_t)c * num_sms(), c);
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess) t.at[c] = n * c;
+      }
+      cudaGetLastError();  // a size that does not fit is a 0 here, not an error
+    });
+    return t.at;
+  }
+
+  static int launch(const LkPageAttnDesc& d, cudaStream_t s) {
+    const int rows = d.Hq / d.Hkv * d.q_len, tiles = cdiv(rows, 8 * NT);
+    const int64_t blocks = (int64_t)d.num_seqs * d.Hkv * tiles * d.nsplit;
+    LK_REQUIRE(blocks < (1ll << 31) && (int64_t)d.num_seqs * d.q_len * d.Hq < (1ll << 31),
+               "page_attention: too many rows in one call");
+    if (places()[0] == 0) return check_launch("page_attention: kernel attributes") ? -1 : fail("page_attention: no room for a block");
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    config(cfg, attr, blocks, d.nsplit);
+    cfg.stream = s;
+    cudaLaunchKernelEx(&cfg, page_attn_kernel<KV, DH, NT>, d,
+                       PaDivs{FastDiv(d.nsplit), FastDiv(d.Hkv), FastDiv(tiles), FastDiv(d.Hq / d.Hkv), FastDiv(d.page)});
+    if (check_launch("page_attention")) return -1;
+    if (d.nsplit <= PA_CLUSTER) return 0;
+    // launched while the parts still run (its blocks wait for them in the launch order of
+    // the stream): the launch's own latency is not waited for
+    cfg.gridDim = dim3((unsigned)((int64_t)d.num_seqs * d.q_len * d.Hq));
+    cfg.blockDim = dim3(32 * JOIN_WARPS);
+    cfg.dynamicSmemBytes = 0;
+    attr = cudaLaunchAttribute{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, page_attn_join_kernel<DH>, d, 8 * NT, d.nsplit);
+    return check_launch("page_attention_join");
   }
-  cudaLaunchKernelEx(&cfg, k, d, PaDivs{FastDiv(d.nsplit), FastDiv(d.Hkv), FastDiv(tiles), FastDiv(d.Hq / d.Hkv), FastDiv(d.page)});
-  if (check_launch("page_attention")) return -1;
-  if (d.nsplit == 1 || cluster) return 0;
-  const int64_t joins = (int64_t)d.num_seqs * d.q_len * d.Hq;
-  // launched while the parts still run (its blocks wait for them in the launch order of
-  // the stream): the launch's own latency is not waited for
-  cfg.gridDim = dim3((unsigned)joins);
-  cfg.blockDim = dim3(32 * JOIN_WARPS);
-  cfg.dynamicSmemBytes = 0;
-  attr = cudaLaunchAttribute{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, page_attn_join_kernel<DH>, d, 8 * NT, d.nsplit);
-  return check_launch("page_attention_join");
+};
+
+template <typename F>  // f(PaKernel of these types and sizes)
+static auto page_attn_variant(int kv_dtype, int Dh, int64_t rows, F f) {
+#define LK_PA(KV, DH) (rows > 8 ? f(PaKernel<KV, DH, 2>()) : f(PaKernel<KV, DH, 1>()))
+  if (kv_dtype == 1) return Dh == 64 ? LK_PA(1, 64) : LK_PA(1, 128);
+  return Dh == 64 ? LK_PA(2, 64) : LK_PA(2, 128);
+#undef LK_PA
 }
 
 }  // namespace lk
@@ -679,48 +718,52 @@ using namespace lk;
 
 // Into how many parts a context may be cut, and the least units of a part, from the
 // longest context that the host expects (each block cuts its sequence's own length).
-// The estimate, in tokens that an SM takes at its full rate:
-//   a part and what a block costs beside it (150 tokens: 2.3 us shared by the blocks of
-//   an SM), times the parts of an SM - half of the time the fullest SM decides (equal
-//   lengths), half the mean, of lengths that are 0.6 of the longest;
-//   but no less than the longest part alone, at the 60 % of the rate that one block reaches;
-//   60 more for the join of a cluster, 300 for a second launch.
-// Measured (us on the device; uncut, chosen, best of 1 to 16 parts): one sequence of 2000
-// tokens 16.3, 6.7, 6.7; 8 of up to 4096 35, 13.8, 13.7; 32 of them 42, 35, 35; 64 of them 62,
-// 62, 59; 256 uncut 182. More than 16 parts: one of 30000 19.6 (16 parts 23.6), two of 100003 64.
+// The estimate, in tokens that an SM takes at its full rate (which two blocks reach, one
+// 60 % of it): a part and what a block costs beside it (150 tokens: 2.3 us shared by the
+// blocks of an SM), in waves of as many blocks as are resident at a time in clusters of
+// this size; half of that for equal lengths, half the same work spread evenly for lengths
+// that are 0.6 of the longest, but no less than the longest part alone; and 60 more for
+// the join of a cluster, 300 for a second launch (more than 16 parts).
+// Measured (us on the device, 32 heads on 8 KV heads of 128 where not said: uncut, chosen, the
+// best of 1 to 16 parts): 1 x 2000 15.3, 6.5, 6.5; 1 x 30000 229, 19.1 (over 16 parts), 23.0;
+// 8 x 4096 34.1, 13.2, 13.4; 16 x 4096 35.1, 20.6, 20.5; 32 x 4096 40.5, 33.7, 33.9; 64 x 4096
+// 58.7, 58.6, 57.0; 32 x 500 7.5, 7.6, 7.5; 24 x 2047 (4 heads of 64) 13.9, 10.3, 9.8;
+// 24 new tokens over 2000 20.5, 12.6, 12.8 (21.0 in 6 parts, whose clusters need a second wave).
 // Beyond what fills the GPU only contexts over 4096 are cut, so that one does not run on
 // alone.
-extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units) {
+extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx,
+                                         int* nsplit, int* min_units) {
   const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
-  const int sms = num_sms(), most = max_ctx <= 768 ? 1 : cdiv(max_ctx, 256);
-  const int full = (int)std::min<int64_t>(most, 3 * (int64_t)sms / blocks + 1), step = std::max(1, full / 32);
+  const int sms = num_sms(), most = max_ctx <= 256 ? 1 : cdiv(max_ctx, 256);
+  const int* places = page_attn_variant(kv_dtype, Dh, rows, [](auto k) { return decltype(k)::places(); });
+  const int full = (int)std::min<int64_t>(most, places[0] / blocks + 1), step = std::max(1, full / 32);
   int best = 1;
   double least = 1e30;
+  auto wave = [&](double part, double held) {  // blocks of an SM: held
+    return part * held / std::min(1.0, 0.6 * held);
+  };
   auto consider = [&](int64_t ns) {
     if (ns < 1 || ns > full) return;
-    const double part = (double)max_ctx / ns + 150, mean = 0.6 * blocks * ns / sms;
-    const double cost = std::max(part * 0.5 * ((double)((blocks * ns + sms - 1) / sms) + mean), part / 0.6) +
-                        (ns > PA_CLUSTER ? 300 : ns > 1 ? 60 : 0);
+    const int64_t all = blocks * ns, room = std::max(1, ns <= PA_CLUSTER ? places[ns] : places[0]) / ns * ns;
+    if (room == 0) return;
+    const double part = (double)max_ctx / ns + 150;
+    const int64_t waves = all / room, rest = all % room;
+    const double even = waves * wave(part, (double)room / sms) + (rest ? wave(part, (double)((rest + sms - 1) / sms)) : 0.0);
+    const double mixed = num_seqs > 1 ? std::max(0.6 * part * all / sms, part / 0.6) : even;
+    const double cost = 0.5 * (even + mixed) + (ns > PA_CLUSTER ? 300 : ns > 1 ? 60 : 0);
     if (cost < least) least = cost, best = (int)ns;
   };
-  for (int ns = 1; ns <= full; ns += step) consider(ns);
+  for (int ns = 1; ns <= std::min(full, PA_CLUSTER); ++ns) consider(ns);
+  for (int ns = PA_CLUSTER + 1; ns <= full; ns += step) consider(ns);
   for (int k = 1; k <= 3; ++k) consider((int64_t)k * sms / blocks);
-  consider(PA_CLUSTER);
   *nsplit = best > 1 ? best : std::max(1, cdiv(max_ctx, 4096));
-  *min_units = best > 1 ? 256 / PA_UNIT : 4096 / PA_UNIT;
+  *min_units = best > 1 ? PA_WARPS : 4096 / PA_UNIT;
 }
 
 extern "C" int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s) {
   LK_REQUIRE(d->Dh == 64 || d->Dh == 128, "page_attention: head_dim must be 64 or 128");
   if (d->num_seqs == 0) return 0;
   LK_REQUIRE(d->nsplit <= PA_CLUSTER || (d->part_o && d->part_ml), "page_attention: split partial buffers needed");
-  const bool wide = d->Hq / d->Hkv * d->q_len > 8;
-#define LK_PA(KV, DH) return wide ? launch_page_attn<KV, DH, 2>(*d, s) : launch_page_attn<KV, DH, 1>(*d, s)
-  if (d->kv_dtype == 1) {
-    if (d->Dh == 64) LK_PA(1, 64);
-    LK_PA(1, 128);
-  }
-  if (d->Dh == 64) LK_PA(2, 64);
-  LK_PA(2, 128);
-#undef LK_PA
+  return page_attn_variant(d->kv_dtype, d->Dh, (int64_t)(d->Hq / d->Hkv) * d->q_len,
+                           [&](auto k) { return decltype(k)::launch(*d, s); });
 }

@@ -498,7 +498,8 @@ typedef struct LkPageAttnDesc {
   int kv_dtype;
   int* status;
 } LkPageAttnDesc;
-void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int max_ctx, int* nsplit, int* min_units);
+void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx, int* nsplit,
+                              int* min_units);
 int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s);
 
 // Copies page moves[2i] over page moves[2i+1] in every layer of every tensor
