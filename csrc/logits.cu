@@ -46,7 +46,7 @@ struct AdjGroup {
 // 5 blocks an SM and blocks of 512 are 2-15 us slower.
 // VEC: every row of every table starts on 16 bytes; a thread takes 8 neighbouring
 // columns at a time.  Otherwise (an odd vocabulary without a padded pitch) its 8 lie a
-// block's width apart, one access each.
+// block's width apart, one access each: 128 rows of 128251 in 40.6 us, of 128256 in 18.8.
 template <typename T, bool VEC, int G>
 __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2) ? 6 : 3) adjust_logits_kernel(LkAdjustLogitsDesc d) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2)
       if (row >= 0) a = *reinterpret_cast<const uint4*>(counts + col(s, 0));
       g.c[0] = a.x, g.c[1] = a.y, g.c[2] = a.z, g.c[3] = a.w;
       g.allowed = mrow >= 0 ? reinterpret_cast<const uint8_t*>(mask)[col(s, 0) / 8] : 0xFFu;
-    } else {
+    } else if (VEC) {  // the end of a row
       g.allowed = 0;
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
@@ -97,6 +97,25 @@ __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2)
         if constexpr (F32) g.x[k] = xw[0], g.x[k + 1] = xw[1];
         else g.x[k / 2] = xw[0] | xw[1] << 16;
         g.c[k / 2] = cw[0] | cw[1] << 16;
+      }
+    } else {
+      // columns past the end ask for the last one again: no branch between the loads
+      uint32_t x[8], c[8], w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int j = min(col(s, k), n - 1);
+        if constexpr (F32) x[k] = __float_as_uint(in[j]);
+        else x[k] = __bfloat16_as_ushort(in[j]);
+        c[k] = row >= 0 ? (uint16_t)counts[j] : 0;
+        w[k] = mrow >= 0 ? (uint32_t)mask[j / 32] : ~0u;
+      }
+      g.allowed = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        g.allowed |= (w[k] >> (col(s, k) & 31) & 1) << k;
+        if (k & 1) g.c[k / 2] = c[k - 1] | c[k] << 16;
+        if constexpr (F32) g.x[k] = x[k];
+        else if (k & 1) g.x[k / 2] = x[k - 1] | x[k] << 16;
       }
     }
     return g;
@@ -285,8 +304,8 @@ extern "C" int lk_adjust_logits(const LkAdjustLogitsDesc* d, cudaStream_t s) {
   const bool vec = rows_aligned(d->logits, d->ld, each, d->n) && rows_aligned(d->out, d->ldo, each, d->n) &&
                    (!d->counts || rows_aligned(d->counts, d->ldc, 2, d->count_rows));
   // two groups a thread share the search for a row's biases and have more loads on their way,
-  // one fills the GPU sooner (us with 1 / 2 groups, 300 biases a row, 128256 columns: 1 row 2.6 /
-  // 3.1, 8 rows 3.6 / 3.4, 16 rows 4.9 / 4.4, 64 rows 12.1 / 9.8)
+  // one fills the GPU sooner (us with 1 / 2 groups, 300 biases a row, 128256 columns: 1 row 2.8 /
+  // 2.9, 16 rows 4.9 / 4.3, 48 rows 9.8 / 8.0; 128251 columns: 3.1 / 4.1, 7.7 / 7.7, 18.2 / 17.0)
   const int groups = (int64_t)d->n * cdiv(d->vocab, ADJ_GROUPS * ADJ_STEP) >= 2 * num_sms() ? ADJ_GROUPS : 1;
   const dim3 grid(cdiv(d->vocab, groups * ADJ_STEP), d->n);
   const int smem = d->bias_offsets ? groups * (ADJ_STEP + ADJ_STEP / 32) * 4 : 0;
