@@ -31,6 +31,7 @@ from collections import deque
 from dataclasses import dataclass, field, replace
 from typing import Callable, Dict, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ..config import ServeConfig, TransformerConfig
@@ -54,7 +55,8 @@ class SamplingParams:
     # output, - frequency * count - presence for generated ones, + bias per token id,
     # and -inf for all but the allowed tokens: a fixed set, or a grammar called with
     # the tokens generated so far (it returns the ids allowed next, None = all; none at
-    # all ends the request with reason "stop" and without a token)
+    # all ends the request with reason "stop" and without a token; an exception or an id
+    # outside the vocabulary ends it with reason "error", Request.error says why)
     repetition_penalty: float = 1.0
     frequency_penalty: float = 0.0
     presence_penalty: float = 0.0
@@ -78,6 +80,15 @@ class SamplingParams:
             return self.allowed_token_ids if ids is None else ids
         fixed = set(self.allowed_token_ids)
         return [t for t in ids if t in fixed]
+
+
+def _token_ids(ids, vocab: int) -> np.ndarray:
+    """Token ids (any iterable of integers, a set among them) as int64 [n]; ValueError where one
+    is no id of the vocabulary."""
+    a = np.asarray(ids if isinstance(ids, (list, tuple, np.ndarray)) else list(ids))
+    if a.size and not (a.ndim == 1 and a.dtype.kind in "iu" and a.min() >= 0 and a.max() < vocab):
+        raise ValueError(f"token ids must be integers in [0, {vocab})")
+    return a.astype(np.int64, copy=False).reshape(-1)
 
 
 def _mix64(a: int, b: int) -> int:
@@ -113,6 +124,7 @@ class Request:
     token_times: List[float] = field(default_factory=list)
     finished: bool = False
     finish_reason: Optional[str] = None
+    error: Optional[str] = None  # what went wrong (finish_reason "error")
     on_token: Optional[Callable[["Request", int], None]] = None
     samples: List[int] = field(default_factory=list)  # ids of the other samples (params.n > 1)
     counts_row: int = -1        # row of the runner's token counts
@@ -202,10 +214,12 @@ class LLMEngine:
                 and p.repetition_penalty < float("inf")):
             raise ValueError("penalties must be finite, repetition_penalty above 0")
         V = self.cfg.vocab_size
-        if any(not 0 <= t < V for t in p.logit_bias or ()) or any(not 0 <= t < V for t in p.allowed_token_ids or ()):
+        if any(not 0 <= t < V for t in p.logit_bias or ()):
             raise ValueError(f"logit_bias and allowed_token_ids take token ids in [0, {V})")
-        if p.allowed_token_ids is not None and not len(p.allowed_token_ids):
-            raise ValueError("allowed_token_ids must not be empty")
+        if p.allowed_token_ids is not None:
+            if not len(p.allowed_token_ids):
+                raise ValueError("allowed_token_ids must not be empty")
+            _token_ids(p.allowed_token_ids, V)
         if not 1 <= p.n <= self.sc.max_num_seqs:
             raise ValueError(f"n must be in [1, {self.sc.max_num_seqs}]")
 
@@ -353,8 +367,8 @@ class LLMEngine:
 
     # ---------------------------------------------------------------- step
     def _emit(self, r: Request, tok: Optional[int], now: float) -> None:
-        if tok is None:  # its grammar allows no token
-            r.finished, r.finish_reason = True, "stop"
+        if tok is None:  # its grammar allows no token, or failed
+            r.finished, r.finish_reason = True, "stop" if r.error is None else "error"
             self._release(r)
             self.running.remove(r)
             self.finished[r.req_id] = r
@@ -395,11 +409,13 @@ class LLMEngine:
             [self._packed_bias(r) for r in reqs], [self._packed_mask(r, a) for r, a in zip(reqs, allowed)])
 
     def _packed_mask(self, r: Request, allowed):
-        pack = getattr(self.runner, "pack_allowed", None)
-        if allowed is None or pack is None or r.params.grammar is not None:
-            return allowed
+        if allowed is None:
+            return None
+        pack = getattr(self.runner, "pack_allowed", None) or np.ndarray.tolist
+        if r.params.grammar is not None:
+            return pack(allowed)
         if r.fixed_mask is None:
-            r.fixed_mask = pack(allowed)
+            r.fixed_mask = pack(_token_ids(allowed, self.cfg.vocab_size))
         return r.fixed_mask
 
     def _packed_bias(self, r: Request):
@@ -410,8 +426,20 @@ class LLMEngine:
             r.fixed_bias = pack(r.params.logit_bias)
         return r.fixed_bias
 
+    def _allowed(self, r: Request) -> Optional[Sequence[int]]:
+        """The token ids that may come next (None = all; an array where a grammar names them).  A grammar is the caller's code: where it
+        fails, its request alone ends (_emit), without a token."""
+        if r.params.grammar is None:
+            return r.params.allowed_token_ids
+        try:
+            ids = r.params.allowed(r.output)
+            return None if ids is None else _token_ids(ids, self.cfg.vocab_size)
+        except Exception as e:
+            r.error = f"grammar: {type(e).__name__}: {e}"
+            return _token_ids((), 0)
+
     def _sample(self, reqs: List[Request], logits: torch.Tensor) -> List[Optional[int]]:
-        allowed = [r.params.allowed(r.output) if r.params.adjusts else None for r in reqs]
+        allowed = [self._allowed(r) for r in reqs]
         tok = self._draw(reqs, self._adjust(reqs, logits, allowed))
         if any(r.counts_row >= 0 for r in reqs):
             self.runner.add_counts([r.counts_row for r in reqs], tok)

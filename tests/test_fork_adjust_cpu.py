@@ -253,6 +253,68 @@ def test_validator_with_adjustments():
             v.check([1], body)
 
 
+def _raises(out):
+    raise RuntimeError("no such state")
+
+
+@pytest.mark.parametrize("grammar,why", [(_raises, "RuntimeError: no such state"), (lambda out: [1, V], "token ids"), (lambda out: [-1], "token ids"),
+                                         (lambda out: [0.5], "token ids"), (lambda out: 7, "TypeError")])
+def test_a_failing_grammar_ends_its_own_request_only(grammar, why):
+    eng, _ = _engine(max_num_seqs=8)
+    late = SamplingParams(max_tokens=9, grammar=lambda out: None if len(out) < 4 else grammar(out), presence_penalty=0.5)
+    ids = [eng.add_request([3, 4, 5], SamplingParams(max_tokens=9)), eng.add_request([3, 4, 5], SamplingParams(max_tokens=9, grammar=grammar)),
+           eng.add_request([6, 7], late), eng.add_request([8, 9], SamplingParams(max_tokens=9, n=2, grammar=grammar))]
+    _run(eng, ids)
+    _run(eng, eng.finished[ids[3]].samples)
+    assert eng.finished[ids[0]].output == reference([3, 4, 5], 9) and eng.finished[ids[0]].error is None
+    for i, n in ((ids[1], 0), (ids[2], 4), (ids[3], 0), (eng.finished[ids[3]].samples[0], 0)):
+        r = eng.finished[i]
+        assert r.finish_reason == "error" and why in r.error and len(r.output) == n
+    assert not eng.has_work() and eng.blocks.num_free() == 64 and sorted(eng._counts_free) == list(range(eng._counts_rows))
+
+
+def test_grammars_may_return_any_collection_of_ids():
+    """Lists, tuples, sets, ranges, generators and arrays alike; a set of fixed ids too."""
+    import numpy as np
+    want = {9, 27, 81}
+    outs = []
+    for kw in (dict(allowed_token_ids=want), dict(allowed_token_ids=np.array([9, 27, 81])), dict(grammar=lambda out: want), dict(grammar=lambda out: tuple(want)),
+               dict(grammar=lambda out: (t for t in want)), dict(grammar=lambda out: np.array([9, 27, 81], dtype=np.int32)),
+               dict(grammar=lambda out: range(9, 82), allowed_token_ids=want), dict(grammar=lambda out: None, allowed_token_ids=want)):
+        eng, _ = _engine()
+        i = eng.add_request([1, 2], SamplingParams(max_tokens=6, **kw))
+        _run(eng, [i])
+        outs.append(eng.finished[i].output)
+    assert all(o == _penalised([1, 2], 6, SamplingParams(allowed_token_ids=[9, 27, 81])) for o in outs)
+
+
+class PackingRunner(Runner):
+    """Takes masks as the words that its pack_allowed makes, as the GPU runner does."""
+
+    def pack_allowed(self, ids):
+        import numpy as np
+        assert isinstance(ids, np.ndarray) and ids.dtype == np.int64
+        bits = np.zeros((V + 31) // 32 * 32, dtype=np.uint8)
+        bits[ids] = 1
+        return np.packbits(bits, bitorder="little").view(np.int32)
+
+    def adjust_logits(self, logits, rows, penalties, biases, allowed):
+        import numpy as np
+        for a in allowed:
+            assert a is None or (a.dtype == np.int32 and a.shape == ((V + 31) // 32,))
+        ids = [None if a is None else np.flatnonzero(np.unpackbits(a.view(np.uint8), bitorder="little")) for a in allowed]
+        return super().adjust_logits(logits, rows, penalties, biases, ids)
+
+
+def test_grammar_arrays_are_ids_not_mask_words():
+    import numpy as np
+    for words in (np.array([5, 6, 7, 8]), np.array([5, 6, 7, 8], dtype=np.int32), {5, 6, 7, 8}):
+        eng, _ = _engine(cls=PackingRunner)
+        i = eng.add_request([1, 2], SamplingParams(max_tokens=4, grammar=lambda out: words[len(out):len(out) + 1] if isinstance(words, np.ndarray) else words))
+        _run(eng, [i])
+        assert set(eng.finished[i].output) <= {5, 6, 7, 8} and eng.finished[i].finish_reason == "length"
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
