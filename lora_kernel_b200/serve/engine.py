@@ -126,6 +126,7 @@ class Request:
     finish_reason: Optional[str] = None
     error: Optional[str] = None  # what went wrong (finish_reason "error")
     on_token: Optional[Callable[["Request", int], None]] = None
+    on_finish: Optional[Callable[["Request"], None]] = None  # called once, however the request ends
     samples: List[int] = field(default_factory=list)  # ids of the other samples (params.n > 1)
     counts_row: int = -1        # row of the runner's token counts
     # params.allowed_token_ids (without a grammar) and logit_bias as the runner packs them, once
@@ -183,7 +184,10 @@ class LLMEngine:
 
     # ---------------------------------------------------------- requests
     def add_request(self, prompt: List[int], params: Optional[SamplingParams] = None, priority: int = 0,
-                    on_token=None, arrival: Optional[float] = None) -> int:
+                    on_token=None, arrival: Optional[float] = None, on_finish=None) -> int:
+        """Queue a prompt; returns the request's id.  on_token(request, token) is called for each token,
+        on_finish(request) once when the request has ended, which it can do without another token (an abort,
+        a grammar that allows none).  Its further samples (params.n > 1) call both too."""
         if not prompt:
             raise ValueError("empty prompt")
         if len(prompt) + (params.max_tokens if params else 16) > self.sc.max_model_len:
@@ -197,7 +201,7 @@ class LLMEngine:
         if params is not None:
             self._check_params(params)
         r = Request(next(self.ids), list(prompt), params or SamplingParams(), priority,
-                    self.clock() if arrival is None else arrival, on_token=on_token)
+                    self.clock() if arrival is None else arrival, on_token=on_token, on_finish=on_finish)
         self.stats["prompt_tokens"] += len(prompt)
         # priority first (lower value = sooner), FIFO within a priority: every
         # request, priority 0 included, goes in front of the first waiting
@@ -231,21 +235,25 @@ class LLMEngine:
             if r.req_id == req_id:
                 self._release(r)
                 self.running.remove(r)
-                r.finished, r.finish_reason = True, "abort"
-                self.finished[r.req_id] = r
+                self._finish(r, "abort")
                 return True
         for r in list(self.waiting):
             if r.req_id == req_id:
                 if r.table:
                     self.blocks.free_seq(r.table)
                 self.waiting.remove(r)
-                r.finished, r.finish_reason = True, "abort"
-                self.finished[r.req_id] = r
+                self._finish(r, "abort")
                 return True
         return False
 
+    def _finish(self, r: Request, reason: Optional[str]) -> None:
+        r.finished, r.finish_reason = True, reason
+        self.finished[r.req_id] = r
+        if r.on_finish:
+            r.on_finish(r)
+
     # ------------------------------------------------------------ forks, pages
-    def fork_request(self, req_id: int, params: Optional[SamplingParams] = None, on_token=None) -> int:
+    def fork_request(self, req_id: int, params: Optional[SamplingParams] = None, on_token=None, on_finish=None) -> int:
         """Continue a running request a second time from where it is now: a new
         request with the same tokens so far, whose KV blocks are shared with the
         first's (the partly filled one copied).  params: the new one's (default:
@@ -259,9 +267,9 @@ class LLMEngine:
             if len(r.prompt) + params.max_tokens > self.sc.max_model_len:
                 raise ValueError("prompt + max_tokens exceeds max_model_len")
             self._check_params(params)
-        return self._fork(r, r.n_tokens - 1, params, on_token).req_id
+        return self._fork(r, r.n_tokens - 1, params, on_token, on_finish).req_id
 
-    def _fork(self, r: Request, computed: int, params: Optional[SamplingParams], on_token) -> Request:
+    def _fork(self, r: Request, computed: int, params: Optional[SamplingParams], on_token, on_finish) -> Request:
         """A copy of r whose first `computed` tokens are in the cache; it runs at once
         where there is room, else it waits and is recomputed (from the prefix cache)."""
         rid = next(self.ids)
@@ -269,7 +277,7 @@ class LLMEngine:
             seed = None if r.params.seed is None else _mix64(r.params.seed, rid) >> 1
             params = replace(r.params, n=1, seed=seed)
         c = Request(rid, list(r.prompt), params, r.priority, self.clock(), output=list(r.output),
-                    cached_prefix=computed, on_token=on_token, first_token_time=r.first_token_time,
+                    cached_prefix=computed, on_token=on_token, on_finish=on_finish, first_token_time=r.first_token_time,
                     token_times=list(r.token_times))
         if hasattr(self.runner, "copy_pages") and len(self.running) < self.sc.max_num_seqs:
             try:
@@ -368,10 +376,9 @@ class LLMEngine:
     # ---------------------------------------------------------------- step
     def _emit(self, r: Request, tok: Optional[int], now: float) -> None:
         if tok is None:  # its grammar allows no token, or failed
-            r.finished, r.finish_reason = True, "stop" if r.error is None else "error"
             self._release(r)
             self.running.remove(r)
-            self.finished[r.req_id] = r
+            self._finish(r, "stop" if r.error is None else "error")
             return
         r.output.append(tok)
         r.token_times.append(now)
@@ -387,7 +394,7 @@ class LLMEngine:
         if r.finished:
             self._release(r)
             self.running.remove(r)
-            self.finished[r.req_id] = r
+            self._finish(r, r.finish_reason)
 
     def _adjust(self, reqs: List[Request], logits: torch.Tensor, allowed: List) -> torch.Tensor:
         """Penalties, biases and masks of the requests that have any; a request new to
@@ -514,7 +521,7 @@ class LLMEngine:
             rows.append(k)
             if r.params.n > 1 and not r.samples:
                 for _ in range(r.params.n - 1):
-                    c = self._fork(r, r.prefill_len, None, r.on_token)
+                    c = self._fork(r, r.prefill_len, None, r.on_token, r.on_finish)
                     r.samples.append(c.req_id)
                     if c.table:
                         out.append(c)

@@ -315,6 +315,24 @@ def test_grammar_arrays_are_ids_not_mask_words():
         assert set(eng.finished[i].output) <= {5, 6, 7, 8} and eng.finished[i].finish_reason == "length"
 
 
+def test_on_finish_is_called_once_however_a_request_ends():
+    """With a last token, without any, aborted while it waits and while it runs, and for each of several samples."""
+    eng, _ = _engine(max_num_seqs=4)
+    ended = []
+    add = lambda **kw: eng.add_request([3, 4, 5], SamplingParams(max_tokens=6, **kw), on_finish=lambda r: ended.append((r.req_id, r.finish_reason, len(r.output))))  # noqa: E731
+    a, b, c, d = add(), add(grammar=lambda out: [] if len(out) == 2 else None), add(grammar=_raises), add(n=2)
+    e, f = add(), add()
+    eng.abort_request(f)
+    eng.step()
+    g = eng.fork_request(a, on_finish=lambda r: ended.append((r.req_id, r.finish_reason, len(r.output))))
+    eng.abort_request(a)
+    _run(eng, [a, b, c, d, e, f, g])
+    _run(eng, eng.finished[d].samples)
+    assert sorted(ended) == sorted([(a, "abort", 1), (b, "stop", 2), (c, "error", 0), (d, "length", 6), (eng.finished[d].samples[0], "length", 6),
+                                    (e, "length", 6), (f, "abort", 0), (g, "length", 6)])
+    assert all(r.finished for r in eng.finished.values()) and eng.blocks.num_free() == 64
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
