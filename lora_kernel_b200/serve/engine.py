@@ -128,6 +128,7 @@ class Request:
     on_token: Optional[Callable[["Request", int], None]] = None
     on_finish: Optional[Callable[["Request"], None]] = None  # called once, however the request ends
     samples: List[int] = field(default_factory=list)  # ids of the other samples (params.n > 1)
+    forks: int = 0              # continuations made of this request, its samples among them
     counts_row: int = -1        # row of the runner's token counts
     # params.allowed_token_ids (without a grammar) and logit_bias as the runner packs them, once
     fixed_mask: Optional[object] = None
@@ -273,8 +274,10 @@ class LLMEngine:
         """A copy of r whose first `computed` tokens are in the cache; it runs at once
         where there is room, else it waits and is recomputed (from the prefix cache)."""
         rid = next(self.ids)
+        r.forks += 1
         if params is None:
-            seed = None if r.params.seed is None else _mix64(r.params.seed, rid) >> 1
+            # another seed for each, the same ones whenever the request is made again
+            seed = None if r.params.seed is None else _mix64(r.params.seed, r.forks) >> 1
             params = replace(r.params, n=1, seed=seed)
         c = Request(rid, list(r.prompt), params, r.priority, self.clock(), output=list(r.output),
                     cached_prefix=computed, on_token=on_token, on_finish=on_finish, first_token_time=r.first_token_time,

@@ -333,6 +333,21 @@ def test_on_finish_is_called_once_however_a_request_ends():
     assert all(r.finished for r in eng.finished.values()) and eng.blocks.num_free() == 64
 
 
+def test_seeded_samples_and_forks_repeat():
+    """Every sample and fork of a seeded request draws with a seed of its own, the same one whatever else the engine served before."""
+    def seeds(busy):
+        eng, _ = _engine(max_num_seqs=8)
+        for k in range(busy):
+            _run(eng, [eng.add_request([k + 1], SamplingParams(max_tokens=2))])
+        i = eng.add_request([1, 2, 3], SamplingParams(max_tokens=6, temperature=1.0, seed=7, n=3))
+        eng.step()
+        kids = next(r for r in eng.running if r.req_id == i).samples + [eng.fork_request(i), eng.fork_request(i)]
+        _run(eng, [i] + kids)
+        return [eng.finished[k].params.seed for k in [i] + kids]
+    first = seeds(0)
+    assert seeds(3) == first and first[0] == 7 and len(set(first)) == 5 and all(0 <= s < 2 ** 63 for s in first)
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
