@@ -193,12 +193,6 @@ class LLMEngine:
             raise ValueError("empty prompt")
         if len(prompt) + (params.max_tokens if params else 16) > self.sc.max_model_len:
             raise ValueError("prompt + max_tokens exceeds max_model_len")
-        if params is not None and params.temperature > 0 and not getattr(self.runner, "supports_top_p", False):
-            if params.top_p < 1.0:
-                raise ValueError("top_p < 1 is not supported by this runner (tensor-parallel serving samples "
-                                 "from vocabulary slices); use top_p = 1")
-            if params.seed is not None:
-                raise ValueError("per-request seeds are not supported by this runner (tensor-parallel serving)")
         if params is not None:
             self._check_params(params)
         r = Request(next(self.ids), list(prompt), params or SamplingParams(), priority,
@@ -212,6 +206,12 @@ class LLMEngine:
         return r.req_id
 
     def _check_params(self, p: SamplingParams) -> None:
+        if p.temperature > 0 and not getattr(self.runner, "supports_top_p", False):
+            if p.top_p < 1.0:
+                raise ValueError("top_p < 1 is not supported by this runner (tensor-parallel serving samples "
+                                 "from vocabulary slices); use top_p = 1")
+            if p.seed is not None:
+                raise ValueError("per-request seeds are not supported by this runner (tensor-parallel serving)")
         if p.adjusts and not getattr(self.runner, "supports_adjust", False):
             raise ValueError("penalties, biases and grammars are not supported by this runner (tensor-parallel serving "
                              "samples from vocabulary slices)")
@@ -258,7 +258,7 @@ class LLMEngine:
         """Continue a running request a second time from where it is now: a new
         request with the same tokens so far, whose KV blocks are shared with the
         first's (the partly filled one copied).  params: the new one's (default:
-        the same with another seed)."""
+        the same with another seed; its max_tokens counts the tokens so far too)."""
         r = next((x for x in self.running if x.req_id == req_id), None)
         if r is None or r.in_prefill or not r.output:
             raise ValueError("fork_request: the request is not running, or has no token yet")
@@ -267,6 +267,8 @@ class LLMEngine:
                 raise ValueError("fork_request: n must be 1")
             if len(r.prompt) + params.max_tokens > self.sc.max_model_len:
                 raise ValueError("prompt + max_tokens exceeds max_model_len")
+            if params.max_tokens <= len(r.output):
+                raise ValueError(f"fork_request: max_tokens counts the {len(r.output)} tokens generated so far")
             self._check_params(params)
         return self._fork(r, r.n_tokens - 1, params, on_token, on_finish).req_id
 

@@ -348,6 +348,33 @@ def test_seeded_samples_and_forks_repeat():
     assert seeds(3) == first and first[0] == 7 and len(set(first)) == 5 and all(0 <= s < 2 ** 63 for s in first)
 
 
+@pytest.mark.parametrize("kw", [dict(temperature=1.0, top_p=0.9), dict(temperature=1.0, seed=4), dict(logit_bias={1: 1.0})])
+def test_fork_request_refuses_what_add_request_refuses(kw):
+    """A runner without top_p, seeds and logits changes: refused at the fork, not inside a step; the first request goes on."""
+    eng, _ = _engine(cls=KVRunner)
+    i = eng.add_request([1, 2, 3], SamplingParams(max_tokens=6))
+    eng.step()
+    for add in (lambda p: eng.add_request([1], p), lambda p: eng.fork_request(i, p)):
+        with pytest.raises(ValueError, match="not supported"):
+            add(SamplingParams(max_tokens=6, **kw))
+    _run(eng, [i])
+    assert eng.finished[i].output == reference([1, 2, 3], 6) and not eng.has_work()
+
+
+def test_fork_request_keeps_to_max_tokens():
+    """max_tokens bounds a fork's whole output: a fork that has it already is refused."""
+    eng, _ = _engine()
+    i = eng.add_request([1, 2, 3], SamplingParams(max_tokens=9))
+    for _ in range(4):
+        eng.step()
+    have = len(next(r for r in eng.running if r.req_id == i).output)
+    with pytest.raises(ValueError, match="max_tokens"):
+        eng.fork_request(i, SamplingParams(max_tokens=have))
+    j = eng.fork_request(i, SamplingParams(max_tokens=have + 1))
+    _run(eng, [i, j])
+    assert eng.finished[j].output == reference([1, 2, 3], have + 1) and eng.finished[i].output == reference([1, 2, 3], 9)
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
