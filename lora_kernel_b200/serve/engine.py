@@ -295,7 +295,9 @@ class LLMEngine:
                 c.scheduled_time = c.arrival
                 self.running.append(c)
                 return c
-        self.waiting.appendleft(c)
+        # ahead of its own priority's requests (its prompt is in the prefix cache), behind lower values
+        idx = next((k for k, w in enumerate(self.waiting) if w.priority >= c.priority), len(self.waiting))
+        self.waiting.insert(idx, c)
         return c
 
     def compact(self) -> int:

@@ -375,6 +375,19 @@ def test_fork_request_keeps_to_max_tokens():
     assert eng.finished[j].output == reference([1, 2, 3], have + 1) and eng.finished[i].output == reference([1, 2, 3], 9)
 
 
+def test_a_fork_that_waits_keeps_its_priority():
+    eng, _ = _engine(max_num_seqs=2)
+    a = eng.add_request([1, 2, 3], SamplingParams(max_tokens=30), priority=1)
+    b = eng.add_request([4, 5, 6], SamplingParams(max_tokens=30), priority=1)
+    for _ in range(3):
+        eng.step()
+    queued = {p: eng.add_request([7, 8], SamplingParams(max_tokens=3), priority=p) for p in (0, 1, 2)}
+    c = eng.fork_request(a)
+    assert [r.req_id for r in eng.waiting] == [queued[0], c, queued[1], queued[2]]
+    _run(eng, [a, b, c] + list(queued.values()))
+    assert eng.finished[c].output == reference([1, 2, 3], 30)
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
