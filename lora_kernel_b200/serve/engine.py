@@ -281,9 +281,10 @@ class LLMEngine:
             # another seed for each, the same ones whenever the request is made again
             seed = None if r.params.seed is None else _mix64(r.params.seed, r.forks) >> 1
             params = replace(r.params, n=1, seed=seed)
-        c = Request(rid, list(r.prompt), params, r.priority, self.clock(), output=list(r.output),
-                    cached_prefix=computed, on_token=on_token, on_finish=on_finish, first_token_time=r.first_token_time,
-                    token_times=list(r.token_times))
+        # a sample of the prompt arrived with it; a fork midway arrives now, and its latencies are
+        # those of its own tokens (the tokens so far have no time in it)
+        c = Request(rid, list(r.prompt), params, r.priority, self.clock() if r.output else r.arrival, output=list(r.output),
+                    cached_prefix=computed, on_token=on_token, on_finish=on_finish)
         if hasattr(self.runner, "copy_pages") and len(self.running) < self.sc.max_num_seqs:
             try:
                 c.table, copies = self.blocks.fork(r.table, computed)
@@ -292,7 +293,7 @@ class LLMEngine:
             else:
                 self.runner.copy_pages(copies)
                 c.prefill_len = c.computed = computed
-                c.scheduled_time = c.arrival
+                c.scheduled_time = c.arrival if r.output else r.scheduled_time
                 self.running.append(c)
                 return c
         # ahead of its own priority's requests (its prompt is in the prefix cache), behind lower values

@@ -388,6 +388,28 @@ def test_a_fork_that_waits_keeps_its_priority():
     assert eng.finished[c].output == reference([1, 2, 3], 30)
 
 
+def test_times_of_samples_and_forks():
+    """Queue time, time to first token and token times of each are its own: none negative, none from before it arrived."""
+    eng, _ = _engine(max_num_seqs=3)
+    now = [0.0]
+    eng.clock = lambda: now[0]
+    i = eng.add_request([1, 2, 3], SamplingParams(max_tokens=6, n=2))
+    now[0] = 1.0
+    eng.step()
+    now[0] = 2.0
+    eng.step()
+    now[0] = 3.0
+    kids = next(r for r in eng.running if r.req_id == i).samples + [eng.fork_request(i), eng.fork_request(i)]  # the last one waits
+    while any(k not in eng.finished for k in [i] + kids):
+        now[0] += 1.0
+        eng.step()
+    for k, arrived, own in ((i, 0.0, 6), (kids[0], 0.0, 6), (kids[1], 3.0, 4), (kids[2], 3.0, 4)):
+        r = eng.finished[k]
+        assert r.output == reference([1, 2, 3], 6) and r.arrival == arrived and len(r.token_times) == own
+        assert r.arrival <= r.scheduled_time <= r.first_token_time == r.token_times[0] and r.token_times == sorted(r.token_times)
+    assert eng.finished[kids[0]].first_token_time == eng.finished[i].first_token_time == 1.0
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
