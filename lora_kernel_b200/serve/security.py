@@ -87,9 +87,11 @@ class InputValidator:
             raise ValidationError("n must be 1 (one choice per request)")
         if self.adjust:
             self._check_adjust(body)
-        for k in ("presence_penalty", "frequency_penalty"):
-            if not self.adjust and body.get(k, 0) not in (0, 0.0, None):
-                raise ValidationError(f"{k} is not supported (use 0)")
+        else:
+            for k in ("presence_penalty", "frequency_penalty"):
+                if body.get(k, 0) not in (0, 0.0, None):
+                    raise ValidationError(f"{k} is not supported (use 0)")
+            refuse_adjustments(body)
         if body.get("logprobs") not in (None, False, 0):
             raise ValidationError("logprobs are not returned by this server")
         pr = body.get("priority", 0)
@@ -108,6 +110,16 @@ class InputValidator:
             if not isinstance(seqs, list) or len(seqs) > 4 or \
                     not all(isinstance(x, str) and 0 < len(x) <= 256 for x in seqs):
                 raise ValidationError("stop must be a string or a list of at most 4 non-empty strings")
+
+
+def refuse_adjustments(body: dict) -> None:
+    """For servers that do not change logits: an answer that ignored these fields would be another request's."""
+    if body.get("repetition_penalty") not in (None, 1):
+        raise ValidationError("repetition_penalty is not supported (use 1)")
+    if body.get("logit_bias") not in (None, {}):
+        raise ValidationError("logit_bias is not supported")
+    if body.get("allowed_token_ids") is not None:
+        raise ValidationError("allowed_token_ids is not supported")
 
 
 def _number(x) -> bool:

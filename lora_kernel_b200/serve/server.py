@@ -42,7 +42,7 @@ from ..utils.logging import get_logger, log_fields
 from ..utils.metrics import REGISTRY, AlertManager, AlertRule, DeviceMetrics
 from .engine import LLMEngine, SamplingParams
 from .security import (AuditLog, ConnectionLimiter, InputValidator, PIIMasker, RequestSigner, RoleAccess,
-                       sanitize_text)
+                       refuse_adjustments, sanitize_text)
 from .tokenizer import ByteTokenizer
 
 log = get_logger("lora_kernel.serve")
@@ -272,7 +272,7 @@ def create_app(engine: LLMEngine, model_name: str = "lora-kernel-b200", api_keys
     keys = set(api_keys)
     adjust = all(getattr(getattr(e, "runner", None), "supports_adjust", False) for e in engines)
     validator = validator or InputValidator(engine.cfg.vocab_size, adjust=adjust)
-    adjust = adjust and getattr(validator, "adjust", False)  # a validator that does not check these fields: they are not read
+    adjust = adjust and getattr(validator, "adjust", False)  # a validator that does not check these fields: they are refused
     masker = PIIMasker() if pii_filter else None
     signer = RequestSigner(signing_secret) if signing_secret else None
 
@@ -343,6 +343,7 @@ def create_app(engine: LLMEngine, model_name: str = "lora-kernel-b200", api_keys
 
     def _adjustments(body) -> dict:
         if not adjust:
+            refuse_adjustments(body)
             return {}
         bias = {int(k): float(v) for k, v in (body.get("logit_bias") or {}).items()}
         return dict(repetition_penalty=float(body.get("repetition_penalty") or 1.0),

@@ -410,6 +410,46 @@ def test_times_of_samples_and_forks():
     assert eng.finished[kids[0]].first_token_time == eng.finished[i].first_token_time == 1.0
 
 
+REFUSED = [{"repetition_penalty": 1.1}, {"logit_bias": {"7": 5}}, {"allowed_token_ids": [1, 2]}, {"allowed_token_ids": []}, {"logit_bias": [1]}]
+NEUTRAL = [{"repetition_penalty": 1.0}, {"repetition_penalty": None, "logit_bias": {}, "allowed_token_ids": None}, {"logit_bias": None}]
+
+
+def test_validator_without_adjustments_refuses_them():
+    v = InputValidator(100)
+    for body in NEUTRAL:
+        v.check([1], body)
+    for body in REFUSED + [{"presence_penalty": 0.5}, {"frequency_penalty": -0.5}]:
+        with pytest.raises(ValidationError, match="not supported"):
+            v.check([1], body)
+
+
+@pytest.mark.parametrize("own_validator", [False, True])
+def test_server_without_adjustments_refuses_them(own_validator):
+    """Over HTTP, chat and the WebSocket, with the server's validator and with one of the caller's that knows nothing of these fields."""
+    from test_server_cpu import _run as serve
+
+    class Lenient:
+        def check(self, ids, body):
+            pass
+
+    async def go(client):
+        for body in REFUSED:
+            r = await client.post("/v1/completions", json={"prompt": "ab", "max_tokens": 2, **body})
+            assert r.status == 400 and "not supported" in (await r.json())["error"]["message"]
+            r = await client.post("/v1/chat/completions", json={"messages": [{"role": "user", "content": "a"}], "max_tokens": 2, **body})
+            assert r.status == 400
+        for body in NEUTRAL:
+            r = await client.post("/v1/completions", json={"prompt": "ab", "max_tokens": 2, **body})
+            assert r.status == 200 and len((await r.json())["token_ids"]) == 2
+        ws = await client.ws_connect("/v1/ws")
+        await ws.send_json({"prompt": "ab", "max_tokens": 2, "allowed_token_ids": [5]})
+        assert "not supported" in (await ws.receive_json())["error"]["message"]
+        await ws.send_json({"prompt": "ab", "max_tokens": 1})
+        assert "token" in await ws.receive_json()
+        await ws.close()
+    serve(go, **({"validator": Lenient()} if own_validator else {}))
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
