@@ -73,6 +73,11 @@ class SamplingParams:
     def adjusts(self) -> bool:
         return self.penalised or bool(self.logit_bias) or self.allowed_token_ids is not None or self.grammar is not None
 
+    @property
+    def banned(self) -> List[int]:
+        """Tokens with a bias of -inf."""
+        return [t for t, b in (self.logit_bias or {}).items() if b < -3.4028235e38]
+
     def allowed(self, output: List[int]) -> Optional[Sequence[int]]:
         """The token ids that may come next (None = all)."""
         ids = self.grammar(output) if self.grammar is not None else None
@@ -215,16 +220,21 @@ class LLMEngine:
         if p.adjusts and not getattr(self.runner, "supports_adjust", False):
             raise ValueError("penalties, biases and grammars are not supported by this runner (tensor-parallel serving "
                              "samples from vocabulary slices)")
-        if not (p.repetition_penalty > 0 and abs(p.frequency_penalty) < float("inf") and abs(p.presence_penalty) < float("inf")
-                and p.repetition_penalty < float("inf")):
-            raise ValueError("penalties must be finite, repetition_penalty above 0")
+        # the kernel's numbers are fp32, and it multiplies by the reciprocal of the repetition penalty
+        most = float(np.finfo(np.float32).max)
+        if not (2.0 ** -126 <= p.repetition_penalty <= 2.0 ** 126 and abs(p.frequency_penalty) <= most and abs(p.presence_penalty) <= most):
+            raise ValueError("penalties must be finite in fp32, repetition_penalty in [2^-126, 2^126]")
+        if not all(b <= most for b in (p.logit_bias or {}).values()):  # -inf bans a token
+            raise ValueError("logit_bias: values must be finite in fp32, or -inf")
         V = self.cfg.vocab_size
         if any(not 0 <= t < V for t in p.logit_bias or ()):
             raise ValueError(f"logit_bias and allowed_token_ids take token ids in [0, {V})")
         if p.allowed_token_ids is not None:
             if not len(p.allowed_token_ids):
                 raise ValueError("allowed_token_ids must not be empty")
-            _token_ids(p.allowed_token_ids, V)
+            ids = _token_ids(p.allowed_token_ids, V)
+            if p.banned and set(ids.tolist()) <= set(p.banned):
+                raise ValueError("logit_bias bans every token of allowed_token_ids")
         if not 1 <= p.n <= self.sc.max_num_seqs:
             raise ValueError(f"n must be in [1, {self.sc.max_num_seqs}]")
 
@@ -448,7 +458,11 @@ class LLMEngine:
             return r.params.allowed_token_ids
         try:
             ids = r.params.allowed(r.output)
-            return None if ids is None else _token_ids(ids, self.cfg.vocab_size)
+            if ids is None:
+                return None
+            ids = _token_ids(ids, self.cfg.vocab_size)
+            banned = r.params.banned
+            return ids[~np.isin(ids, banned)] if banned else ids  # banned ones are no choice: none left ends the request
         except Exception as e:
             r.error = f"grammar: {type(e).__name__}: {e}"
             return _token_ids((), 0)

@@ -450,6 +450,22 @@ def test_server_without_adjustments_refuses_them(own_validator):
     serve(go, **({"validator": Lenient()} if own_validator else {}))
 
 
+def test_values_outside_fp32_are_refused():
+    """What fp32 turns into 0, infinity or NaN would spoil a row of logits; -inf bans a token."""
+    eng, _ = _engine()
+    for kw in (dict(repetition_penalty=1e-50), dict(repetition_penalty=1e39), dict(repetition_penalty=2.0 ** -127), dict(repetition_penalty=float("nan")),
+               dict(frequency_penalty=1e39), dict(presence_penalty=-1e39), dict(logit_bias={3: float("nan")}), dict(logit_bias={3: float("inf")}),
+               dict(logit_bias={3: 1e39}), dict(logit_bias={3: -float("inf"), 4: -float("inf")}, allowed_token_ids=[4, 3, 4])):
+        with pytest.raises(ValueError):
+            eng.add_request([1], SamplingParams(**kw))
+    ban = -float("inf")
+    for kw, want in ((dict(logit_bias={9: ban}, allowed_token_ids=[9, 27]), [27] * 4), (dict(logit_bias={9: ban, 27: ban}, grammar=lambda out: [9, 27]), []),
+                     (dict(logit_bias={9: ban}, grammar=lambda out: [9, 27] if len(out) < 2 else [9]), [27, 27])):
+        i = eng.add_request([1, 2], SamplingParams(max_tokens=4, **kw))
+        _run(eng, [i])
+        assert eng.finished[i].output == want and eng.finished[i].finish_reason == ("length" if len(want) == 4 else "stop")
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
