@@ -18,7 +18,14 @@ KV caches: each model keeps the KV of a prefix of the committed tokens.  A
 round feeds the draft the committed tokens it has not seen plus its own
 proposals, and feeds the target the unseen committed tokens plus the k
 proposals with logits for every row.  Rejected positions are dropped by
-truncating the cached length; their stale KV is overwritten later.
+truncating the cached length; their stale KV is overwritten later.  In a cache
+with one scale per page they can have raised the scale of the page that the
+kept tokens end in, which rounds those tokens' codes again: RunnerScorer then
+computes the kept tokens of that page once more with the next ones, so that the
+page holds what it would have held without them.  While a round is scored, its
+proposals do share a page with the tokens before them, so over such a cache the
+target's own greedy decode is met up to the rounding of the codes (int8: up to a
+bit per doubling of the scale; e4m3: codes that become subnormal).
 
 `Scorer` is the interface to a model: `RunnerScorer` drives a `ModelRunner`
 (the paged-KV serving runner; one sequence, contiguous KV slots), and any
@@ -65,6 +72,8 @@ class RunnerScorer(Scorer):
             raise ValueError("RunnerScorer: a page-scaled cache needs a base slot at the start of a page")
         self.seq_id = seq_id
         self._len = 0
+        self._tokens: List[int] = []  # the cached positions' tokens (kept for page-scaled caches)
+        self._valid = 0               # positions below this are in the cache as they should be
 
     @property
     def length(self) -> int:
@@ -75,14 +84,25 @@ class RunnerScorer(Scorer):
         n = len(tokens)
         if self._len + n > self.max_len:
             raise ValueError("RunnerScorer: sequence longer than its slot range")
+        again = self._tokens[self._valid:self._len]  # empty unless rows of their page were dropped
         slots = list(range(self.base, self.base + self._len + n))
-        item = PrefillItem(self.seq_id, list(tokens), self._len, slots, True, all_logits)
+        item = PrefillItem(self.seq_id, again + list(tokens), self._len - len(again), slots, True, all_logits)
         _, logits = self.runner.prefill([item])
+        if self._paged:
+            self._tokens[self._len:] = tokens
         self._len += n
-        return logits.float()
+        self._valid = self._len
+        return (logits[-n:] if all_logits else logits).float()
+
+    @property
+    def _paged(self) -> bool:
+        return getattr(self.runner, "page_scaled", False)
 
     def truncate(self, length: int) -> None:
-        self._len = min(self._len, length)
+        if length < self._len:
+            self._len = length
+            start = length - length % self.runner.block_size if self._paged else length
+            self._valid = min(self._valid, start)
 
 
 @dataclass

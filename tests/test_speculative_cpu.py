@@ -95,3 +95,50 @@ def test_speculative_sampling_matches_target_distribution():
     e = want * runs
     chi2 = float(((counts - e) ** 2 / e).sum())
     assert chi2 < 25.0, (counts / runs, want)  # 4 dof: p ~ 5e-5
+
+
+class PageRunner:
+    """Keeps what an append does to a page's scale: offset 0 starts the page afresh, later rows can only raise it."""
+
+    def __init__(self, page_scaled, block_size=8, num_blocks=8):
+        self.page_scaled, self.block_size, self.num_blocks, self.max_model_len = page_scaled, block_size, num_blocks, block_size * num_blocks
+        self.slot, self.scale, self.rows = {}, {}, 0
+
+    def prefill(self, items):
+        (it,) = items
+        assert it.want_logits and len(it.slots) == it.start + len(it.tokens)
+        for t, s in zip(it.tokens, it.slots[it.start:]):
+            page, off = divmod(s, self.block_size)
+            self.scale[page] = t if off == 0 else max(self.scale[page], t)
+            self.slot[s] = t
+        self.rows += len(it.tokens)
+        seen = [self.slot[s] for s in it.slots]
+        n = len(it.tokens) if it.all_logits else 1
+        return [it.seq_id], torch.tensor([[float(sum(seen[:len(seen) - n + k + 1])), float(len(seen) - n + k)] for k in range(n)])
+
+
+@pytest.mark.parametrize("page_scaled", [True, False])
+@pytest.mark.parametrize("prompt,drafts,keep", [(5, 2, 1), (8, 3, 0), (13, 12, 1), (13, 12, 3), (20, 5, 4), (20, 5, 5), (3, 20, 14), (1, 1, 0)])
+def test_dropped_rows_leave_no_trace_in_a_page(page_scaled, prompt, drafts, keep):
+    """After truncate and the next rows, tokens, page scales and logits are those of a sequence that never had the dropped rows."""
+    from lora_kernel_b200.serve.speculative import RunnerScorer
+    a, b = PageRunner(page_scaled), PageRunner(page_scaled)
+    sa, sb = RunnerScorer(a, base_slot=16, max_len=48), RunnerScorer(b, base_slot=16, max_len=48)
+    d = list(range(100, 100 + drafts))
+    for s in (sa, sb):
+        s.extend(list(range(1, prompt + 1)), False)
+    sa.extend(d, True)
+    sa.truncate(prompt + keep)
+    assert sa.length == prompt + keep
+    if keep:
+        sb.extend(d[:keep], True)
+    for nxt, every in (([3, 4, 5], True), ([6], False)):
+        la, lb = sa.extend(nxt, every), sb.extend(nxt, every)
+        assert torch.equal(la, lb) and sa.length == sb.length
+    pages = {s // 8 for s in range(16, 16 + sa.length)}
+    assert {p: a.scale[p] for p in pages} == {p: b.scale[p] for p in pages} or not page_scaled
+    assert all(a.slot[s] == b.slot[s] for s in range(16, 16 + sa.length))
+    if not page_scaled:
+        assert a.rows == prompt + drafts + 4  # nothing is computed twice
+    sa.truncate(0)
+    assert sa.length == 0 and torch.equal(sa.extend([9, 9], True), torch.tensor([[9.0, 0.0], [18.0, 1.0]]))
