@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
     for (int s = 0; s <= PA_STAGES; ++s) pg[s] = page_of(warp + s * PA_WARPS);
   }
   // query fragments: column r of each tile, the dims of this lane's key bytes, times
-  // a power of two that brings the tile's largest value to [2^14, 2^15): f16 then
+  // a power of two of its own that brings the row's largest value to [2^14, 2^15): f16 then
   // holds a bf16 value exactly down to 2^-31 of it, and 2^-39 of it is the rounding
   uint32_t qf[NT][4 * CH][2];
 #pragma unroll
@@ -287,20 +287,23 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
   Place pg_next = pg[R::STAGES];
 
   int lim[NT][2];
-  float amax = 0.f;
+  float qfac[NT][2];  // of this lane's score columns 2c and 2c + 1
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n) {
+    float amax = 0.f;  // of row r of the tile, whose dims its four lanes hold
 #pragma unroll
     for (int i = 0; i < 8 * CH; ++i) {
       const float2 f = unpack_bf16x2(qf[n][i / 2][i % 2]);
       if (fabsf(f.x) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.x));
       if (fabsf(f.y) <= 3.4028234e38f) amax = fmaxf(amax, fabsf(f.y));
     }
-  const int e = max((int)(__float_as_uint(warp_max(amax)) >> 23) - 127 - 14, -112);
-  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-  const float qfac = __uint_as_float((uint32_t)(127 + e) << 23) * (d.scale * 1.4426950408889634f);
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -112);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23) * (d.scale * 1.4426950408889634f);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+    for (int q = 0; q < 2; ++q) qfac[n][q] = __shfl_sync(0xffffffffu, up, (2 * c + q) * 4);
 #pragma unroll
     for (int k = 0; k < 4 * CH; ++k)
 #pragma unroll
@@ -363,12 +366,12 @@ __global__ void __launch_bounds__(32 * PA_WARPS, NT == 1 ? (DH == 64 ? 4 : 3) : 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float2 sc = *reinterpret_cast<const float2*>(st + R::SCALES + (16 * g + 8 * i + r) * 8);
-        const float kf = sc.x * qfac, lv = __log2f(sc.y);
+        const float lv = __log2f(sc.y);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            s[g][n][2 * i + q] *= kf;
+            s[g][n][2 * i + q] *= sc.x * qfac[n][q];
             x[g][n][2 * i + q] = s[g][n][2 * i + q] + lv;
           }
       }

@@ -311,6 +311,27 @@ def test_attention_nan_query_and_future_tokens():
     assert torch.equal(out[:2], base[:2]) and not torch.equal(out[2], base[2])
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("Hq,Hkv,Dh,q_len", [(4, 1, 64, 1), (4, 1, 128, 3), (8, 2, 64, 5), (1, 1, 128, 7)])
+def test_attention_query_rows_far_apart(kind, Hq, Hkv, Dh, q_len):
+    """Query rows (heads, tokens) 2^30 to 2^120 above their neighbours in a tile: the others keep their bits."""
+    page, ctxs = 16, [70, 333]
+    (k, v, ks, vs), bt, refs = _filled(kind, ctxs, page, Hkv, Dh, 91)
+    g = torch.Generator(device=dev).manual_seed(92)
+    q = torch.randn(2 * q_len, Hq, Dh, device=dev, generator=g).to(torch.bfloat16)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=dev)
+
+    def call(x):
+        return P().page_attention(x.view(2 * q_len, Hq * Dh), k, v, ks, vs, bt, ctx, page, Hq, Hkv, Dh, q_len=q_len).view(2 * q_len, Hq, Dh)
+
+    base = call(q)
+    _check_attention(base, q, refs, ctxs, q_len, Hq, Dh)
+    big = torch.arange(2 * q_len * Hq, device=dev).view(2 * q_len, Hq) % 3 == 1
+    for e in (30, 60, 120):
+        out = call(torch.where(big[:, :, None], q * 2.0 ** e, q))
+        assert torch.equal(out[~big], base[~big])
+
+
 def test_attention_reports_bad_page_ids():
     """A page id outside the cache is recorded, its tokens are left out, nothing is read there."""
     Hq, Hkv, Dh, page = 4, 1, 64, 16
