@@ -170,3 +170,33 @@ def test_speculative_decoding_over_pages():
     with pytest.raises(ValueError):
         RunnerScorer(eng.runner, base_slot=8)
     _status_ok()
+
+
+@pytest.mark.parametrize("kv", ["fp8_page", "int8_page"])
+def test_rejected_rows_leave_no_trace_in_a_page(kv):
+    """Rows dropped by truncate do not raise the scale of the page that the kept ones end in: scales and logits are those
+    of a sequence that never had them.  (A page's largest value may differ by the roundings of another chunk size, some
+    percent after three layers: scales whose bound is nearer than that are left out.)"""
+    from lora_kernel_b200.serve.speculative import RunnerScorer
+    _, _, ea = _engine(kv)
+    _, _, eb = _engine(kv)
+    a, b = RunnerScorer(ea.runner), RunnerScorer(eb.runner)
+    drafts = _tokens(1, 12) + [999] * 12
+    for s in (a, b):
+        s.runner.W["embed"][999] = s.runner.W["layers.0.wqkv"][8 * 64]  # a token with a large key (layer 0, head 0, dim 0)
+        s.extend(_tokens(50, 11, 999), False)
+    a.extend(drafts, True)
+    raised = float(ea.runner.k_scale[0, 3, 0])
+    a.truncate(51)
+    b.extend(drafts[:1], True)
+    la, lb = a.extend(_tokens(3, 13, 999), True), b.extend(_tokens(3, 13, 999), True)
+    assert la.shape == lb.shape == (3, 1000) and a.length == b.length == 54
+    q = {"fp8_page": 448.0, "int8_page": 127.0}[kv]
+    assert raised >= 2 * float(eb.runner.k_scale[0, 3, 0]) == 2 * float(ea.runner.k_scale[0, 3, 0])
+    for sa, sb, codes in ((ea.runner.k_scale, eb.runner.k_scale, eb.runner.k_cache), (ea.runner.v_scale, eb.runner.v_scale, eb.runner.v_cache)):
+        assert torch.equal(sa[:, :3], sb[:, :3])
+        filled = codes[:, 48:54].float().abs().amax(dim=(1, 3)) / q  # of the page's largest value, 1/2 to 1
+        clear = (filled > 0.54) & (filled < 0.95)
+        assert torch.equal(sa[:, 3][clear], sb[:, 3][clear])
+    assert ((la - lb).norm() / lb.norm()).item() < 5e-2
+    _status_ok()
