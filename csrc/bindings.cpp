@@ -1265,7 +1265,7 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
   d.status = status.data_ptr<int>();
   if (max_ctx <= 0 || max_ctx > tables.size(1) * page) max_ctx = tables.size(1) * page;
   TORCH_CHECK(max_ctx < (1ll << 31) - 64, "page_attention: contexts of fewer than 2^31 tokens");
-  lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)Dh, d.kv_dtype, (int)max_ctx, &d.nsplit, &d.min_units);
+  d.nsplit = lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)Dh, d.kv_dtype, (int)max_ctx);
   torch::Tensor part;  // allocated per call: the allocator knows the stream
   if (d.nsplit > 16) {
     const int64_t parts = q.size(0) * Hq * d.nsplit;

@@ -166,7 +166,7 @@ __device__ __forceinline__ PaSpan page_attn_span(const LkPageAttnDesc& d, int ct
   s.ctx = (int)min((int64_t)max(ctx, 0), (int64_t)d.max_pages * d.page);
   s.end = max(0, s.ctx - d.q_len + last_token + 1);
   s.units = (s.end + PA_UNIT - 1) / PA_UNIT;
-  s.per = max((s.units + d.nsplit - 1) / d.nsplit, d.min_units);
+  s.per = max((s.units + d.nsplit - 1) / d.nsplit, PA_WARPS);  // a unit for each warp at least
   return s;
 }
 
@@ -719,8 +719,8 @@ static auto page_attn_variant(int kv_dtype, int Dh, int64_t rows, F f) {
 
 using namespace lk;
 
-// Into how many parts a context may be cut, and the least units of a part, from the
-// longest context that the host expects (each block cuts its sequence's own length).
+// Into how many parts a context may be cut, from the longest context that the host expects
+// (each block cuts its sequence's own length).
 // The estimate, in tokens that an SM takes at its full rate (which two blocks reach, one
 // 60 % of it): a part and what a block costs beside it (150 tokens: 2.3 us shared by the
 // blocks of an SM), in waves of as many blocks as are resident at a time in clusters of
@@ -732,10 +732,14 @@ using namespace lk;
 // 8 x 4096 34.1, 13.2, 13.4; 16 x 4096 35.1, 20.6, 20.5; 32 x 4096 40.5, 33.7, 33.9; 64 x 4096
 // 58.7, 58.6, 57.0; 32 x 500 7.5, 7.6, 7.5; 24 x 2047 (4 heads of 64) 13.9, 10.3, 9.8;
 // 24 new tokens over 2000 20.5, 12.6, 12.8 (21.0 in 6 parts, whose clusters need a second wave).
-// Beyond what fills the GPU only contexts over 4096 are cut, so that one does not run on
-// alone.
-extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx,
-                                         int* nsplit, int* min_units) {
+// A batch that fills the GPU by itself is not cut, whatever max_ctx says: in a captured step that
+// is the longest context the server allows, not the batch's.  256 sequences of up to 2000 tokens
+// take 92 us at any max_ctx; cut into parts of 4096 they took 157 us for a max_ctx of 8192 and 619
+// for 32768 (the parts' blocks without tokens hold their places until their cluster is done; 157
+// and 237 if they leave at once, which is what starting them costs).  Uncut, a long context among
+// short ones runs on alone: 30000 tokens beside 255 sequences of up to 500 (2000) 266 (313) us, of
+// which cut in either way 358 (640) and 155 (258).
+extern "C" int lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx) {
   const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
   const int sms = num_sms(), most = max_ctx <= 256 ? 1 : cdiv(max_ctx, 256);
   const int* places = page_attn_variant(kv_dtype, Dh, rows, [](auto k) { return decltype(k)::places(); });
@@ -759,8 +763,7 @@ extern "C" void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hk
   for (int ns = 1; ns <= std::min(full, PA_CLUSTER); ++ns) consider(ns);
   for (int ns = PA_CLUSTER + 1; ns <= full; ns += step) consider(ns);
   for (int k = 1; k <= 3; ++k) consider((int64_t)k * sms / blocks);
-  *nsplit = best > 1 ? best : std::max(1, cdiv(max_ctx, 4096));
-  *min_units = best > 1 ? PA_WARPS : 4096 / PA_UNIT;
+  return best;
 }
 
 extern "C" int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s) {

@@ -492,14 +492,13 @@ typedef struct LkPageAttnDesc {
   float scale;
   void* out;  // [num_seqs * q_len, Hq*Dh] bf16
   int64_t ldo;
-  int nsplit, min_units;  // parts of each context (lk_page_attention_splits)
+  int nsplit;  // parts of each context (lk_page_attention_splits)
   float* part_o;   // [num_seqs * q_len, Hq, nsplit, Dh] when nsplit > 16 (fewer parts join in their cluster)
   float* part_ml;  // [num_seqs * q_len, Hq, nsplit, 4]
   int kv_dtype;
   int* status;
 } LkPageAttnDesc;
-void lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx, int* nsplit,
-                              int* min_units);
+int lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx);
 int lk_page_attention(const LkPageAttnDesc* d, cudaStream_t s);
 
 // Copies page moves[2i] over page moves[2i+1] in every layer of every tensor

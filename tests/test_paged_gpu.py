@@ -246,6 +246,50 @@ def test_attention_parts(kind, Hq, Hkv, Dh, q_len, ctxs):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_attention_full_batch_with_long_bounds(kind):
+    """A batch that fills the GPU, two long contexts in it, with bounds from below the longest to far above it."""
+    Hq, Hkv, Dh, page = 16, 8, 64, 16
+    ctxs = [(37 * i) % 90 for i in range(158)] + [5000, 9001]
+    (k, v, ks, vs), bt, refs = _filled(kind, ctxs, page, Hkv, Dh, 21)
+    q = torch.randn(len(ctxs), Hq * Dh, device=dev, generator=torch.Generator(device=dev).manual_seed(1)).to(torch.bfloat16)
+    ctx = torch.tensor(ctxs, dtype=torch.int32, device=dev)
+    wide = torch.cat([bt, torch.full((len(ctxs), 8192), -1, dtype=torch.int32, device=dev)], dim=1)
+    for table, max_ctx in ((bt, 9001), (bt, 90), (wide, 32768), (wide, 0)):
+        out = P().page_attention(q, k, v, ks, vs, table, ctx, page, Hq, Hkv, Dh, max_ctx=max_ctx)
+        _check_attention(out, q, refs, ctxs, 1, Hq, Dh)
+    assert _status_code() == ""
+
+
+def test_attention_full_batch_takes_no_longer_for_a_longer_bound():
+    """A captured step passes the longest context that the server allows: the same work must not wait for parts without
+    tokens (up to 300 tokens in a batch of 1024 blocks took nine times as long for a bound of 32768)."""
+    Hq, Hkv, Dh, page, n = 32, 8, 128, 16, 128
+    k, v, ks, vs = _cache("fp8_page", 1024, page, Hkv, Dh)
+    ks.fill_(1.0)
+    vs.fill_(1.0)
+    bt = torch.randint(0, 1024, (n, 32768 // page), device=dev, dtype=torch.int32, generator=torch.Generator(device=dev).manual_seed(1))
+    ctx = (torch.arange(n, device=dev) * 7 % 300 + 1).to(torch.int32)
+    q = torch.randn(n, Hq * Dh, device=dev).to(torch.bfloat16)
+
+    def us(max_ctx):
+        best = 1e9
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(20):
+                P().page_attention(q, k, v, ks, vs, bt, ctx, page, Hq, Hkv, Dh, max_ctx=max_ctx)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 50)
+        return best
+
+    us(4096)
+    base = us(4096)
+    for bound in (4097, 8192, 32768):
+        assert us(bound) < 2 * base
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_scales_far_apart(kind):
     """Pages whose values differ by 2^40: a query that looks at a page of small values still sees them."""
     Hq, Hkv, Dh, page, ctxs = 4, 1, 64, 8, [200, 31]
