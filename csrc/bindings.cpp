@@ -1263,8 +1263,11 @@ torch::Tensor page_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tens
   d.scale = (float)scale;
   d.out = out.data_ptr(); d.ldo = out.stride(0);
   d.status = status.data_ptr<int>();
-  if (max_ctx <= 0 || max_ctx > tables.size(1) * page) max_ctx = tables.size(1) * page;
-  TORCH_CHECK(max_ctx < (1ll << 31) - 64, "page_attention: contexts of fewer than 2^31 tokens");
+  // token indexes are ints, and run ahead of a context by the units that are on their way
+  const int64_t most = tables.size(1) * page;
+  TORCH_CHECK(tables.size(1) < (1ll << 31) && page < (1ll << 31) && most < (1ll << 31) - 4096,
+              "page_attention: block_tables must be of fewer than 2^31 - 4096 tokens a sequence");
+  if (max_ctx <= 0 || max_ctx > most) max_ctx = most;
   d.nsplit = lk_page_attention_splits((int)n, (int)q_len, (int)Hq, (int)Hkv, (int)Dh, d.kv_dtype, (int)max_ctx);
   torch::Tensor part;  // allocated per call: the allocator knows the stream
   if (d.nsplit > 16) {

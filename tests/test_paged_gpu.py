@@ -547,6 +547,20 @@ def test_copy_pages_refuses():
 
 
 # ------------------------------------------------------------------ refusals
+def test_tables_of_too_many_tokens_are_refused():
+    """Whatever max_ctx says: a context's end near 2^31 would take token indexes past it."""
+    paged = P()
+    none = torch.empty(0, dtype=torch.int32, device=dev)
+    q = torch.empty(0, 64, dtype=torch.bfloat16, device=dev)
+    for page, width in ((1, 2 ** 31 - 8), (16, 2 ** 27), (64, 2 ** 40)):
+        k, v, ks, vs = _cache("fp8_page", 2, page, 1, 64)
+        for max_ctx in (0, 5):
+            with pytest.raises(RuntimeError, match="block_tables"):
+                paged.page_attention(q, k, v, ks, vs, torch.empty(0, width, dtype=torch.int32, device=dev), none, page, 1, 1, 64, max_ctx=max_ctx)
+        out = paged.page_attention(q, k, v, ks, vs, torch.empty(0, 2 ** 20, dtype=torch.int32, device=dev), none, page, 1, 1, 64, max_ctx=5)
+        assert out.shape == (0, 64)
+
+
 def test_refusals():
     paged = P()
     Hq, Hkv, Dh, page = 4, 2, 64, 16
