@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2)
               p = row >= 0 ? d.penalties[3 * i + 2] : 0.f;
 
   int any = 0;  // a bias falls into this span
+  __shared__ int again;  // two biases fall onto one column
   if (b0 < b1) {
     // ids and values of a thread's first two biases are asked for together and at once:
     // the block lives as long as its longest chain of loads
@@ -141,12 +142,14 @@ __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2)
     }
     constexpr int words = G * (ADJ_STEP + ADJ_STEP / 32) / 4;
     for (int j = tid; j < words; j += ADJ_THREADS) reinterpret_cast<float4*>(extra)[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (tid == 0) again = 0;
     __syncthreads();
     auto add = [&](int token, float x) {
       const int at = token - v0;
       if ((unsigned)at < (unsigned)n) {
-        atomicAdd(&extra[at], x);
-        atomicOr(&biased[at / 32], 1u << (at & 31));
+        const uint32_t bit = 1u << (at & 31);
+        if (atomicOr(&biased[at / 32], bit) & bit) again = 1;
+        else extra[at] = x;
         any = 1;
       } else if (blockIdx.x == 0 && (unsigned)token >= (unsigned)d.vocab && d.status) {
         atomicCAS(d.status, 0, LK_ERR_BAD_INDEX);
@@ -157,6 +160,16 @@ __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2)
       if (b0 + tid + k * ADJ_THREADS < b1) add(id[k], value[k]);
     for (int j = b0 + tid + FIRST * ADJ_THREADS; j < b1; j += ADJ_THREADS) add(d.bias_ids[j], d.bias_values[j]);
     any = __syncthreads_or(any);
+    if (again) {  // an id is named more than once: each thread adds up its own columns in the list's order
+#pragma unroll 1
+      for (int j = tid; j < G * ADJ_STEP; j += ADJ_THREADS) extra[j] = 0.f;
+#pragma unroll 1
+      for (int j = b0; j < b1; ++j) {
+        const int at = d.bias_ids[j] - v0;
+        if ((unsigned)at < (unsigned)n && at % ADJ_THREADS == tid) extra[at] += d.bias_values[j];
+      }
+      __syncthreads();
+    }
   }
 
   const float inv_r = 1.f / r;

@@ -61,7 +61,8 @@ def adjust_logits(logits: torch.Tensor, counts: Optional[torch.Tensor] = None, r
     count being how often it was generated; penalties fp32 [n, 3] holds
     (repetition, frequency, presence).  rows int32 [n]: None = row i, negative
     = no penalties.  Then bias (offsets int32 [n + 1], ids int32, values fp32)
-    is added, and tokens whose bit in mask int32 [m, ceil(vocab / 32)] is 0
+    is added (an id named more than once: its values' sum, in the list's order),
+    and tokens whose bit in mask int32 [m, ceil(vocab / 32)] is 0
     become -inf; mask_rows int32 [n]: None = row i, negative = unrestricted.
     fp32 throughout, rounded once."""
     require_device(logits)

@@ -156,6 +156,27 @@ def test_adjust_in_place_keeps_the_rest_to_the_bit():
         assert torch.equal(got.view(torch.int16)[same], raw[same])
 
 
+@pytest.mark.parametrize("n,vocab", [(1, 3000), (40, 32003)])
+def test_bias_ids_named_several_times(n, vocab):
+    """Their biases add up in fp32 in the order of the list, the same in every call; other columns get their own."""
+    ops = L()
+    g = torch.Generator().manual_seed(5)
+    for many in (2, 3, 600, 1500):
+        ids = torch.cat([torch.full((many,), 77), torch.tensor([vocab - 1, 300, 77 + 256, vocab - 1])]).repeat(n)
+        vals = torch.randn(n, many + 4, generator=g) * 10.0 ** torch.randint(-3, 6, (n, many + 4), generator=g)
+        want = torch.zeros(n, vocab)
+        for i in range(n):
+            for j in range(many):
+                want[i, 77] += vals[i, j]
+            want[i, 300], want[i, 333] = vals[i, many + 1], vals[i, many + 2]
+            want[i, vocab - 1] = vals[i, many] + vals[i, many + 3]
+        bias = ((torch.arange(n + 1) * (many + 4)).to(torch.int32).to(dev), ids.to(torch.int32).to(dev), vals.reshape(-1).to(dev))
+        for _ in range(3):
+            got = ops.adjust_logits(torch.zeros(n, vocab, device=dev), bias=bias)
+            assert torch.equal(got.cpu(), want)
+    assert _status_code() == ""
+
+
 def test_bad_indices_are_reported():
     ops = L()
     z = torch.randn(2, 100, device=dev)
