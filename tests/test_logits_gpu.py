@@ -105,6 +105,41 @@ def test_adjust_logits(dtype, n, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,vocab", [(40, 32003), (40, 32008), (150, 6000), (150, 6001)])
+def test_adjust_logits_of_many_rows(dtype, n, vocab):
+    """Batches whose threads take two groups of columns, rows on and off 16 bytes; a row's last span ends inside the first
+    group (6000) and inside the second (32003)."""
+    ops = L()
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    z = (torch.randn(n, vocab, device=dev, generator=g) * 4).to(dtype)
+    counts = _table(n + 2, vocab, 1)
+    rows = [(7 * i + 3) % (n + 2) if i % 5 else -1 for i in range(n)]
+    pen = torch.rand(n, 3, device=dev, generator=g) + torch.tensor([0.5, -0.3, -0.5], device=dev)
+    # columns 0, 2047, 2048 and the last one among them
+    biases = [{t % vocab: (k - 3) * 1.37 for k, t in enumerate((0, 2047, 2048, 4095, 4096, vocab - 1, 97 * i, 131 * i + 5))} if i % 3 else None
+              for i in range(n)]
+    allowed = torch.rand(n, vocab, device=dev, generator=g) < 0.6
+    mask_rows = [(i + 1) % n if i % 4 else -1 for i in range(n)]
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    for use in (1, 2, 4, 7, 15):
+        kw = {}
+        if use & 1:
+            kw.update(counts=counts, rows=t(rows), penalties=pen)
+        if use & 2:
+            kw.update(bias=ops.logit_bias(biases, dev))
+        if use & 4:
+            kw.update(mask=_bits(allowed), mask_rows=t(mask_rows))
+        target = z.clone()
+        if use & 8:
+            kw["out"] = target  # in place
+        out = ops.adjust_logits(target, **kw)
+        _compare(out, z, counts if use & 1 else None, rows, pen if use & 1 else None, biases if use & 2 else [None] * n,
+                 allowed if use & 4 else None, mask_rows)
+        assert use & 8 or torch.equal(target, z)
+    assert _status_code() == ""
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_adjust_strides_and_identity_rows(dtype):
     """Row pitches of every alignment (logits, counts, masks, output), rows and mask rows left out."""
     ops = L()
