@@ -94,6 +94,42 @@ def test_append_in_pieces(kind, Hq, Hkv, Dh, page):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [1, 7, 16, 40, 256])
+@pytest.mark.parametrize("rows", [600, 2100])
+def test_append_many_rows(kind, page, rows):
+    """Calls whose warps look for runs in windows of several rows: three sequences that go on inside a page (the page's
+    scale grows), skipped rows between them, runs across window borders and longer than a warp looks at once."""
+    paged = P()
+    Hkv, Dh = 1, 64
+    g = torch.Generator(device=dev).manual_seed(page)
+    starts = [0, page // 2, 3 * page + page // 3]
+    takes = [rows // 2, rows // 3, rows - rows // 2 - rows // 3]
+    need = [-(-(s + t) // page) for s, t in zip(starts, takes)]
+    pages = sum(need) + 3
+    k, v, ks, vs = cache = _cache(kind, pages, page, Hkv, Dh)
+    _garbage(cache, 2)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(3)).tolist()
+    tables = [[order.pop() for _ in range(n)] for n in need]
+    cpu = [O.PageCache(c.cpu(), s.cpu(), page) for c, s in ((k, ks), (v, vs))]
+    held = [_slots(t, page, 0, n) for t, n in zip(tables, starts)]
+    new = [_slots(t, page, n, n + m) + [-1] * 3 for t, n, m in zip(tables, starts, takes)]
+    for slots, size in ((sum(held, []), 1.0), (sum(new, []), 4.0)):
+        x = torch.randn(len(slots), 2 * Hkv, Dh, device=dev, generator=g) * size
+        x = (x * torch.exp2(torch.randint(-3, 4, (len(slots), 1, 1), device=dev, generator=g).float())).to(torch.bfloat16)
+        paged.page_append(x.view(len(slots), -1), 0, Hkv, Dh, torch.tensor(slots, dtype=torch.int32, device=dev), k, v, ks, vs, page)
+        cpu[0].append(x[:, :Hkv].cpu(), slots)
+        cpu[1].append(x[:, Hkv:].cpu(), slots)
+    at = torch.tensor(sorted(s for s in sum(held + new, []) if s >= 0))
+    for got, sc, ref in ((k, ks, cpu[0]), (v, vs, cpu[1])):
+        assert torch.equal(got.cpu()[at].double(), ref.codes[at])
+        assert torch.equal(sc.cpu()[at // page].double(), ref.scale[at // page])
+    rest = torch.ones(pages * page, dtype=torch.bool)
+    rest[at] = False
+    assert torch.equal(k.cpu()[rest].double().nan_to_num(7.5), cpu[0].codes[rest].nan_to_num(7.5)), "slots not appended to"
+    assert _status_code() == ""
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_append_edges(kind):
     """Zeros, subnormals, the largest values, infinities and NaN; skipped rows; boundaries of the scale."""
     paged = P()
