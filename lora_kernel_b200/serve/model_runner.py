@@ -15,7 +15,7 @@ cache of every layer and runs two kinds of batches:
 With kv_dtype "fp8_page" / "int8_page" the cache has one power-of-two scale per
 (page, KV head) instead of one per (token, KV head) (ops/paged.py): appends,
 decode attention (tensor cores) and the read-back for prefill go through its
-kernels, and chunks of up to PAGE_ATTN_ROWS tokens (speculative verification, the
+kernels, and chunks of few query rows (page_attn_tokens: speculative verification, the
 end of a prompt whose beginning is cached) attend to the pages directly.
 
 The LM head runs only on each sequence's last row; K19 samples the next token,
@@ -274,10 +274,20 @@ class ModelRunner:
             return SV.sample_topp(logits, t, p, seed, row_seeds=rs)
         return SV.sample(logits, t, seed)
 
-    # A chunk of up to this many rows attends to the pages themselves instead of a bf16 copy
-    # of its context (us, 32 / 8 heads of 128, pages / copy and flash kernel: 16 rows over 2000
-    # tokens 10 / 37, over 8000 31 / 126; 64 rows 30 / 38 and 70 / 126; 128 rows 36 / 40, 97 / 128)
-    PAGE_ATTN_ROWS = 128
+    # A chunk of few query rows attends to the pages themselves instead of a bf16 copy of its
+    # context.  Its cost grows with heads x tokens, a row's about with head_dim + 64; the copy and
+    # the flash kernel cost about the same up to 128 tokens and more.  us, pages / copy and flash:
+    # 32 heads of 128 (on 8), 16 tokens over 2000 11 / 38, over 8000 19 / 126; 64 tokens 20 / 38 and
+    # 52 / 127; 128 tokens 27 / 40 and 90 / 129; 160 tokens 42 / 45 and 142 / 147; 192 tokens 49 / 45 and
+    # 146 / 147.  64 heads of 128, 64 tokens 28 / 39 and 91 / 128; 80 tokens 44 / 39 and 143 / 128.  64 heads
+    # of 64, 96 tokens 26 / 30 and 82 / 95; 128 tokens 36 / 31 and 118 / 95.  8 heads of 64, 512 tokens
+    # 20 / 40 and 62 / 130; 1536 tokens 36 / 40 and 148 / 130.
+    PAGE_ATTN_ROWS = 128  # tokens at 32 heads of 128
+
+    @property
+    def page_attn_tokens(self) -> int:
+        """Longest chunk that attends to the pages."""
+        return self.PAGE_ATTN_ROWS * 32 * (128 + 64) // (self.cfg.num_heads * (self.cfg.head_dim + 64))
 
     # -------------------------------------------------------------- prefill
     @torch.no_grad()
@@ -306,7 +316,7 @@ class ModelRunner:
         pages = [None] * len(items)  # (page table, length) of the chunks that attend to the pages themselves
         if self.page_scaled:
             for k, it in enumerate(items):
-                if it.start > 0 and len(it.tokens) <= self.PAGE_ATTN_ROWS:
+                if it.start > 0 and len(it.tokens) <= self.page_attn_tokens:
                     end = it.start + len(it.tokens)
                     pages[k] = (torch.tensor([[s // bs for s in it.slots[:end:bs]]], dtype=torch.int32, device=dev),
                                 torch.tensor([end], dtype=torch.int32, device=dev))

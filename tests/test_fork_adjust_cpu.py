@@ -466,6 +466,17 @@ def test_values_outside_fp32_are_refused():
         assert eng.finished[i].output == want and eng.finished[i].finish_reason == ("length" if len(want) == 4 else "stop")
 
 
+def test_chunks_that_attend_to_the_pages_are_bounded_by_query_rows():
+    """Heads count as tokens do: the longest such chunk shrinks with them (128 tokens of 64 heads were slower than a copy)."""
+    from types import SimpleNamespace
+    from lora_kernel_b200.serve.model_runner import ModelRunner
+    longest = lambda h, dh, rows=ModelRunner.PAGE_ATTN_ROWS: ModelRunner.page_attn_tokens.fget(  # noqa: E731
+        SimpleNamespace(cfg=SimpleNamespace(num_heads=h, head_dim=dh), PAGE_ATTN_ROWS=rows))
+    assert longest(32, 128) == 128 and longest(64, 128) == 64 and longest(8, 128) == 512
+    assert longest(32, 64) == 192 and longest(64, 64) == 96 and longest(8, 64) == 768
+    assert longest(28, 128) == 146 and longest(32, 128, 0) == 0
+
+
 # ------------------------------------------------------------------ the oracles themselves
 def test_page_oracle_properties():
     import paged_oracle as O
