@@ -1174,6 +1174,11 @@ torch::Tensor empty_beside(const torch::Tensor& like, at::IntArrayRef size, c10:
   return at::detail::empty_cuda(size, dt, like.device(), c10::nullopt);
 }
 
+// Counts that the kernels hold as ints, a grid's last blocks included.
+void int_count(const char* op, const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() <= (1ll << 31) - 4096, op, ": ", name, " must be of fewer than 2^31 - 4096 elements");
+}
+
 void same_device(const char* op, const torch::Tensor& a, std::initializer_list<const torch::Tensor*> others) {
   for (const torch::Tensor* t : others)
     TORCH_CHECK(t->device() == a.device(), op, ": tensors are on ", a.device().str(), " and ", t->device().str());
@@ -1190,6 +1195,7 @@ void page_append(torch::Tensor qkv, int64_t Hq, int64_t Hkv, int64_t Dh, torch::
               "page_append: the rows of qkv must be 16-byte aligned");
   need_contig(slots, "slots", torch::kInt32);
   TORCH_CHECK(slots.numel() == qkv.size(0), "page_append: one slot per row");
+  int_count("page_append", slots, "slots");
   LkPageAppendDesc d{};
   d.kv_dtype = page_cache("page_append", k_cache, v_cache, k_scale, v_scale, Hkv, Dh, page);
   same_device("page_append", qkv, {&slots, &k_cache, &v_cache, &k_scale, &v_scale, &status});
@@ -1208,6 +1214,7 @@ torch::Tensor page_gather(torch::Tensor k_cache, torch::Tensor v_cache, torch::T
                           c10::optional<torch::Tensor> out_opt, torch::Tensor status) {
   const c10::cuda::CUDAGuard g(k_cache.device());
   need_contig(slots, "slots", torch::kInt32);
+  int_count("page_gather", slots, "slots");
   torch::Tensor out = out_opt.has_value() ? *out_opt
                                           : empty_beside(k_cache, {slots.numel(), 2 * Hkv * Dh}, torch::kBFloat16);
   need(out, "out", torch::kBFloat16);
@@ -1285,6 +1292,7 @@ void copy_pages(std::vector<torch::Tensor> caches, torch::Tensor moves, int64_t 
   const c10::cuda::CUDAGuard g(caches[0].device());
   need_contig(moves, "moves", torch::kInt32);
   TORCH_CHECK(moves.dim() == 2 && moves.size(1) == 2, "copy_pages: moves must be [n, 2] (source, destination)");
+  int_count("copy_pages", moves, "moves");
   TORCH_CHECK(num_pages > 0 && num_pages < (1ll << 31), "copy_pages: num_pages");
   LkCopyPagesDesc d{};
   d.layers = (int)caches[0].size(0);
@@ -1355,6 +1363,7 @@ torch::Tensor adjust_logits(torch::Tensor logits, c10::optional<torch::Tensor> c
     need_contig(*bias_values, "bias values", torch::kFloat32);
     TORCH_CHECK(bias_offsets->numel() == n + 1 && bias_ids->numel() == bias_values->numel(),
                 "adjust_logits: bias offsets [n + 1], one value per id");
+    int_count("adjust_logits", *bias_ids, "bias ids");
     same_device("adjust_logits", logits, {&*bias_offsets, &*bias_ids, &*bias_values});
     d.bias_offsets = bias_offsets->data_ptr<int>();
     d.bias_ids = bias_ids->data_ptr<int>();
@@ -1390,6 +1399,7 @@ void set_token_counts(torch::Tensor counts, c10::optional<torch::Tensor> rows, t
   need_contig(prompt_lens, "prompt_lens", torch::kInt32);
   const int64_t n = prompt_lens.numel();
   TORCH_CHECK(offsets.numel() == n + 1, "set_token_counts: offsets [n + 1], prompt_lens [n]");
+  int_count("set_token_counts", tokens, "tokens");
   same_device("set_token_counts", counts, {&tokens, &offsets, &prompt_lens, &status});
   LkTokenCountsDesc d{};
   d.counts = counts.data_ptr<int16_t>(); d.ldc = counts.stride(0);
@@ -1411,6 +1421,7 @@ void add_token_counts(torch::Tensor counts, c10::optional<torch::Tensor> rows, t
   const c10::cuda::CUDAGuard g(counts.device());
   row_table("add_token_counts", counts);
   need_contig(tokens, "tokens", torch::kInt64);
+  int_count("add_token_counts", tokens, "tokens");
   same_device("add_token_counts", counts, {&tokens, &status});
   const int* r = nullptr;
   if (rows.has_value()) {

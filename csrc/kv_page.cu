@@ -278,7 +278,7 @@ extern "C" int lk_page_gather(const LkPageGatherDesc* d, cudaStream_t s) {
   const int per_row = d->Hkv * d->Dh / 8;
   const int64_t total = (int64_t)d->n * per_row;
   if (total == 0) return 0;
-  LK_REQUIRE(total < (1ll << 31), "page_gather: too many rows in one call");
+  LK_REQUIRE(total <= (1ll << 31) - 256, "page_gather: too many rows in one call");  // the last block's items are ints too
   const int grid = cdiv(total, 256);
   if (d->kv_dtype == 1)
     page_gather_kernel<1><<<grid, 256, 0, s>>>(*d, (int)total, FastDiv(per_row), FastDiv(d->page));

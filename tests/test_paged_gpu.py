@@ -583,6 +583,31 @@ def test_copy_pages_refuses():
 
 
 # ------------------------------------------------------------------ refusals
+def test_counts_past_31_bits_are_refused():
+    """Rows, moves, histories and biases whose indexes would pass 31 bits (nothing is launched; 17 GB, never touched)."""
+    from lora_kernel_b200.ops import logits
+    paged = P()
+    k, v, ks, vs = _cache("fp8_page", 2, 16, 1, 64)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+    tokens = torch.empty(2 ** 31, dtype=torch.int64, device=dev)
+    out = torch.empty(1, 128, dtype=torch.bfloat16, device=dev)
+    slots = tokens.view(torch.int32)
+    for n in (2 ** 28 - 1, 2 ** 31 - 4096, 2 ** 31, 2 ** 32):  # the first: items of the last block alone pass 31 bits
+        with pytest.raises(RuntimeError):
+            paged.page_gather(k, v, ks, vs, slots[:n], 1, 64, 16, out=out.expand(n, 128))
+    with pytest.raises(RuntimeError):
+        paged.copy_pages([k[None]], slots.view(-1, 2), 2)
+    counts = torch.zeros(2, 64, dtype=torch.int16, device=dev)
+    with pytest.raises(RuntimeError):
+        logits.set_token_counts(counts, None, tokens, i32(2), i32(1))
+    with pytest.raises(RuntimeError):
+        logits.add_token_counts(counts, slots[:2 ** 31], tokens)
+    with pytest.raises(RuntimeError):
+        logits.adjust_logits(torch.zeros(1, 64, device=dev), bias=(i32(2), slots[:2 ** 31], slots[:2 ** 31].view(torch.float32)))
+    del tokens, slots
+    torch.cuda.empty_cache()
+
+
 def test_tables_of_too_many_tokens_are_refused():
     """Whatever max_ctx says: a context's end near 2^31 would take token indexes past it."""
     paged = P()
