@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(256) page_gather_kernel(LkPageGatherDesc d, in
 }
 
 // ---------------------------------------------------------------- page copies
-// grid (chunks of a page, layers and moves; tensors): PER threads copy PER * 64 bytes of one page
+// grid (items, tensors), an item being a chunk of a page (fastest), a layer, a move: PER threads copy PER * 64 bytes of one page
 // of one layer of one tensor, every load on its way before the first store: a block 8 KB, or
 // a warp 2 KB where pages are no larger (one block each took 47 us for 41600 pages of 256
 // bytes, a warp each 20).  Bound by HBM (1500 pages of 8 KB in 22 layers of two tensors: 169

@@ -7,8 +7,8 @@
 // Query j of a sequence of ctx tokens sits at position ctx - q_len + j.  A query
 // without a token before it (an unused batch row of ctx 0) gives zeros.
 //
-// The cache is read once: 2 * Hkv * Dh bytes a token, against 4 * Hq * Dh flops
-// per query token, so HBM bounds it as long as the work per byte stays small.
+// The cache is read once per tile of 8 or 16 query rows: 2 * Hkv * Dh bytes a token, against
+// 4 * Hq * Dh flops per query token, so HBM bounds it as long as the work per byte stays small.
 // On CUDA cores it does not (conversions, products and the reductions of the
 // scores cost more issue slots than the bytes bring), hence tensor cores, with
 // the tokens as the M dimension of both products so that the few query rows
@@ -33,10 +33,10 @@
 // ones whichever the query looks at.  The softmax sum is kept in fp32 apart.
 //
 // Measured: 256 sequences of up to 4096 tokens (32 / 8 heads of 128, e4m3, 1084 MB)
-// 182-193 us, 86-91 % of the HBM copy rate; two of 100003 tokens 64 us (79 %); int8 codes
-// take two instructions more a pair: 200 us.  A block costs 3.5 us beside its tokens
+// 184-195 us, 85-90 % of the HBM copy rate; two of 100003 tokens 63-66 us (77-80 %); int8 codes
+// take two instructions more a pair: 197 us.  A block costs 3.5 us beside its tokens
 // (launch, length and pages, first data, merge), which is what the full batch lacks, and
-// at head_dim 64 more (65 us for a floor of 42).  Where rows are few, a warp's 480
+// at head_dim 64 more (4 KV heads: 64 us for a floor of 42).  Where rows are few, a warp's 480
 // instructions per 32 tokens and their dependences bound it: 24 sequences of up to 2047
 // tokens with five queries each (40 rows, 8 / 1 heads of 64, int8) 22.5 us.
 #include <algorithm>
@@ -728,17 +728,17 @@ using namespace lk;
 // that are 0.6 of the longest, but no less than the longest part alone; and 60 more for
 // the join of a cluster, 300 for a second launch (more than 16 parts).
 // Measured (us on the device, 32 heads on 8 KV heads of 128 where not said: uncut, chosen, the
-// best of 1 to 16 parts): 1 x 2000 15.3, 6.5, 6.5; 1 x 30000 229, 19.1 (over 16 parts), 23.0;
-// 8 x 4096 34.1, 13.2, 13.4; 16 x 4096 35.1, 20.6, 20.5; 32 x 4096 40.5, 33.7, 33.9; 64 x 4096
-// 58.7, 58.6, 57.0; 32 x 500 7.5, 7.6, 7.5; 24 x 2047 (4 heads of 64) 13.9, 10.3, 9.8;
-// 24 new tokens over 2000 20.5, 12.6, 12.8 (21.0 in 6 parts, whose clusters need a second wave).
+// best of 1 to 16 parts): 1 x 2000 15.7, 6.4, 6.5; 1 x 30000 257, 19.3 (over 16 parts), 23.7;
+// 8 x 4096 36.5, 13.5, 13.4; 16 x 4096 37.3, 21.8, 21.8; 32 x 4096 42.5, 34.9, 34.8; 64 x 4096
+// 60.3, 61.2, 58.1; 32 x 500 7.7, 7.7, 7.7; 24 x 2047 (4 heads of 64, int8) 13.9, 10.3, 10.1;
+// 24 new tokens over 2000 20.0, 12.7, 12.8 (20.9 in 6 parts, whose clusters need a second wave).
 // A batch that fills the GPU by itself is not cut, whatever max_ctx says: in a captured step that
 // is the longest context the server allows, not the batch's.  256 sequences of up to 2000 tokens
-// take 92 us at any max_ctx; cut into parts of 4096 they took 157 us for a max_ctx of 8192 and 619
-// for 32768 (the parts' blocks without tokens hold their places until their cluster is done; 157
-// and 237 if they leave at once, which is what starting them costs).  Uncut, a long context among
-// short ones runs on alone: 30000 tokens beside 255 sequences of up to 500 (2000) 266 (313) us, of
-// which cut in either way 358 (640) and 155 (258).
+// take 95 us at any max_ctx; in parts of 4096 they took 157 us for a max_ctx of 8192 and 619 for
+// 32768 (the parts' blocks without tokens hold their places until their cluster is done), 157 and
+// 237 where such blocks left at once, which is what starting them costs.  Uncut, a long context
+// among short ones runs on alone: 30000 tokens beside 255 sequences of up to 500 (2000) take 288
+// (336) us, against 358 (640) and 155 (258) in those two forms.
 extern "C" int lk_page_attention_splits(int num_seqs, int q_len, int Hq, int Hkv, int Dh, int kv_dtype, int max_ctx) {
   const int64_t rows = (int64_t)(Hq / Hkv) * q_len, blocks = std::max<int64_t>(1, num_seqs * Hkv * (rows <= 8 ? 1 : (rows + 15) / 16));
   const int sms = num_sms(), most = max_ctx <= 256 ? 1 : cdiv(max_ctx, 256);

@@ -42,11 +42,11 @@ struct AdjGroup {
 // column: the logits stay packed, and only pairs of columns with a count or a bias are
 // taken apart (1 % of the columns are seen or biased in a request of some thousand
 // tokens: 40 % of a warp's pairs).  256 rows of 128256 with 300 biases each and masks
-// in 38.2 us, 35 without biases (torch.add of the logits and the counts: 31); 1 or 4 groups,
+// in 38.9 us, 35 without biases (torch.add of the logits and the counts: 31); 1 or 4 groups,
 // 5 blocks an SM and blocks of 512 are 2-15 us slower.
 // VEC: every row of every table starts on 16 bytes; a thread takes 8 neighbouring
 // columns at a time.  Otherwise (an odd vocabulary without a padded pitch) its 8 lie a
-// block's width apart, one access each: 128 rows of 128251 in 40.6 us, of 128256 in 18.8.
+// block's width apart, one access each: 128 rows of 128251 in 44 us, of 128256 in 20.
 template <typename T, bool VEC, int G>
 __global__ void __launch_bounds__(ADJ_THREADS, G == 1 || (VEC && sizeof(T) == 2) ? 6 : 3) adjust_logits_kernel(LkAdjustLogitsDesc d) {
   constexpr bool F32 = sizeof(T) == 4;

@@ -5,7 +5,8 @@ between 1 and k+1 tokens.
 
 Greedy (temperature 0): draft tokens are accepted while they equal the
 target's argmax; the first mismatch is replaced by the target's argmax.  The
-output is token-for-token the target's own greedy decode.
+output is token-for-token the target's own greedy decode (over a page-scaled
+cache up to the rounding described below).
 
 Sampling (temperature > 0), the speculative sampling rule of Leviathan et al.
 2023 / Chen et al. 2023: draft token d_j ~ q_j is accepted with probability
